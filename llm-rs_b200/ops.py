@@ -1925,3 +1925,191 @@ def rglru_step(u: torch.Tensor, w: torch.Tensor, r_bias: torch.Tensor, i_bias: t
         _LL(_row_stride(y, "y")), _ptr(y_bias), _ptr(state), _ptr(ctx.slot_ids), _ptr(out), _LL(out.stride(0)), n, w.size(0),
         w.size(1), _stream()), "rglru_step")
     return out
+
+
+# -- rows and products in 8 bits -------------------------------------------------------------------------
+# Rows of numbers as float8_e4m3fn ``q`` [rows, K], whose rows start at multiples of 16 bytes, and float8_e8m0fnu ``scales``
+# [ceil(K / 512), rows, 4]: element [g, r, j] is the power of two 2^E that multiplies numbers 128 * (4 g + j) .. + 127 of row r, E
+# the least integer >= -127 with which the block's largest magnitude is at most 448. Places past a row's last block hold 2^-127.
+FP8, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+FP8_BLOCK = 128         # numbers of a row that share a scale
+_FP8_WORD = 512         # numbers of a row whose scales are one 32-bit word
+
+
+def _fp8_new(rows: int, K: int, device):
+    """Room for rows in 8 bits: (q, scales, bytes between q's rows)."""
+    pitch = (K + 15) // 16 * 16
+    q = torch.empty((rows, pitch), dtype=FP8, device=device)
+    scales = torch.empty((-(-K // _FP8_WORD), rows, 4), dtype=FP8_SCALE, device=device)
+    return (q if pitch == K else q[:, :K]), scales, pitch
+
+
+def _fp8_on_device(*tensors) -> None:
+    """All on the current CUDA device (a kernel is launched on that device's stream)."""
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise KernelError("tensors must be on a CUDA device (this engine has no CPU path)")
+    at = {t.device.index for t in tensors if t is not None}
+    current = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    if at != {current}:
+        raise KernelError(f"tensors on devices {sorted(at)}, the current device is {current}")
+
+
+def _fp8_rows(x: torch.Tensor, name: str, K: Optional[int] = None) -> int:
+    """The row stride of a matrix of float32 or bfloat16 with dense rows."""
+    if x.dtype not in _DTYPE_CODE:
+        raise KernelError(f"{name}: kernels take float32 or bfloat16, not {x.dtype}")
+    if x.dim() != 2 or x.size(1) < 1:
+        raise KernelError(f"{name} must be [rows, numbers], got {tuple(x.shape)}")
+    if K is not None and x.size(1) != K:
+        raise KernelError(f"{name} has {x.size(1)} columns, expected {K}")
+    return x.size(1) if x.size(0) == 1 else _row_stride(x, name)
+
+
+def _fp8_operand(q: torch.Tensor, scales: torch.Tensor, name: str):
+    """(bytes between rows, words between the scales of neighbouring words) of rows in 8 bits."""
+    if q.dtype != FP8 or scales.dtype != FP8_SCALE:
+        raise KernelError(f"{name} must be {FP8} with scales of {FP8_SCALE}, got {q.dtype} with {scales.dtype}")
+    if q.dim() != 2 or q.size(1) < 1:
+        raise KernelError(f"{name} must be [rows, K], got {tuple(q.shape)}")
+    rows, K = q.shape
+    words = -(-K // _FP8_WORD)
+    if scales.shape != (words, rows, 4):
+        raise KernelError(f"{name} is {tuple(q.shape)}: its scales must be {(words, rows, 4)}, got {tuple(scales.shape)}")
+    if rows == 0:
+        return (K + 15) // 16 * 16, 0
+    pitch = q.stride(0) if rows > 1 else (K + 15) // 16 * 16
+    if (K > 1 and q.stride(1) != 1) or pitch % 16 or pitch < K or q.data_ptr() % 16:
+        raise KernelError(f"{name}: rows must be dense and start at multiples of 16 bytes, got strides {q.stride()}")
+    stride = scales.stride(0) if words > 1 else 4 * rows
+    if scales.stride(2) != 1 or (rows > 1 and scales.stride(1) != 4) or stride % 4 or stride < 0 or scales.data_ptr() % 4:
+        raise KernelError(f"{name}: a word of four scales must be dense, and words of neighbouring rows adjacent, got strides "
+                          f"{scales.stride()}")
+    return pitch, stride // 4
+
+
+def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
+    """Rows of float32 or bfloat16 ``x`` [rows, K] (dense rows, any stride) in 8 bits: ``(q, scales)`` as above, each number
+    rounded once, to nearest. A NaN or an infinity becomes a NaN. ``src`` (int32): row i is made from row ``src[i]`` of x (one row
+    may be named often; an index that names none of x's rows gives zeros). Weights are quantised by the same call."""
+    stride = _fp8_rows(x, "x")
+    rows, K = x.shape
+    if src is not None:
+        if src.dtype != torch.int32 or src.dim() != 1 or not src.is_contiguous():
+            raise KernelError(f"src must be a contiguous int32 vector, got {src.dtype} {tuple(src.shape)}")
+    _fp8_on_device(x, src)
+    n = rows if src is None else src.numel()
+    q, scales, pitch = _fp8_new(n, K, x.device)
+    _check(_lib().llmrs_quantize_fp8(_ptr(x), _DTYPE_CODE[x.dtype], _LL(stride), rows, _ptr(src), _ptr(q), _LL(pitch),
+                                     _ptr(scales), n, K, _stream()), "quantize_fp8")
+    return q, scales
+
+
+def silu_mul_fp8(gate_up: torch.Tensor, block: int = 0, unit=PLAIN_SILU):
+    """``silu_mul`` with its result in 8 bits: ``(q, scales)`` of ``silu(gate) * up`` for ``gate_up`` [rows, 2I] that holds gate and
+    up in alternating runs of ``block`` columns (0: I gate columns, then I up columns; else a divisor of I). The unit is
+    computed in float32 and rounded once."""
+    stride = _fp8_rows(gate_up, "gate_up")
+    rows, two = gate_up.shape
+    inter = two // 2
+    if two % 2 or block < 0 or (block and inter % block):
+        raise KernelError(f"gate_up has {two} columns: not two times a multiple of runs of {block}")
+    _fp8_on_device(gate_up)
+    q, scales, pitch = _fp8_new(rows, inter, gate_up.device)
+    _check(_lib().llmrs_silu_mul_fp8(_ptr(gate_up), _DTYPE_CODE[gate_up.dtype], _LL(stride), block or inter,
+                                     *map(ctypes.c_float, unit), _ptr(q), _LL(pitch), _ptr(scales), rows, inter, _stream()),
+           "silu_mul_fp8")
+    return q, scales
+
+
+def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
+                    rows: Optional[torch.Tensor] = None):
+    """``add_rmsnorm`` with its result in 8 bits: ``h += delta`` (float32 or bfloat16, when given) in place, then ``(q, scales)`` of
+    ``h / sqrt(mean(h^2) + eps) * weight``, rounded once. With ``rows`` (int32) only those rows are normed, into row i, and ``h`` is
+    left as it is; an index that names no row gives zeros."""
+    for name, t in (("h", h), ("weight", weight)):
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise KernelError(f"{name} must be contiguous float32, got {t.dtype}")
+    _fp8_rows(h, "h")
+    n, K = h.shape
+    if weight.numel() != K:
+        raise KernelError(f"norm weight has {weight.numel()} elements, rows have {K}")
+    if delta is not None and (delta.dtype not in _DTYPE_CODE or delta.shape != h.shape or not delta.is_contiguous()):
+        raise KernelError(f"delta {tuple(delta.shape)} ({delta.dtype}) must be float32 or bfloat16 rows like h {tuple(h.shape)}")
+    if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
+        raise KernelError(f"rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
+    _fp8_on_device(h, delta, weight, rows)
+    m = n if rows is None else rows.numel()
+    q, scales, pitch = _fp8_new(m, K, h.device)
+    _check(_lib().llmrs_add_rmsnorm_fp8(_ptr(h), _ptr(delta), BF16 if delta is not None and delta.dtype == torch.bfloat16 else F32,
+                                        _ptr(weight), _ptr(rows), n, ctypes.c_float(eps), _ptr(q), _LL(pitch), _ptr(scales), m, K,
+                                        _stream()), "add_rmsnorm_fp8")
+    return q, scales
+
+
+def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+             out: Optional[torch.Tensor] = None, epilogue: str = "store", out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x @ w.T`` of rows in 8 bits, ``x`` [tokens, K] and ``w`` [features, K] (``quantize_fp8``), on tcgen05 with the scales applied
+    by the tensor core and float32 sums (see csrc/gemm_fp8.cu). Epilogue "store": [tokens, features] in ``out_dtype`` (bfloat16 or
+    float32), into ``out`` when given. "residual": ``out``, the float32 residual stream, gets the product added."""
+    x_pitch, xs = _fp8_operand(x, x_scales, "x")
+    w_pitch, ws = _fp8_operand(w, w_scales, "w")
+    tokens, K = x.shape
+    features = w.size(0)
+    if w.size(1) != K:
+        raise KernelError(f"x has {K} columns, w has {w.size(1)}")
+    if features < 1:
+        raise KernelError("w has no rows")
+    if epilogue not in ("store", "residual"):
+        raise KernelError(f"unknown epilogue {epilogue!r}: 'store' or 'residual'")
+    add = epilogue == "residual"
+    if add and out is None:
+        raise KernelError("the residual epilogue needs the stream it adds to as out")
+    if out is None:
+        dtype_code(out_dtype)
+        _fp8_on_device(x, x_scales, w, w_scales)
+        out = torch.empty((tokens, features), dtype=out_dtype, device=x.device)
+    else:
+        if out.dtype != (torch.float32 if add else out_dtype) or out.shape != (tokens, features):
+            raise KernelError(f"out is {tuple(out.shape)} {out.dtype}, the product {(tokens, features)} "
+                              f"{torch.float32 if add else out_dtype}")
+        dtype_code(out.dtype)
+        _row_stride(out, "out")
+        _fp8_on_device(x, x_scales, w, w_scales, out)
+    _check(_lib().llmrs_gemm_fp8(_ptr(x), _LL(x_pitch), _ptr(x_scales), _LL(xs), tokens, _ptr(w), _LL(w_pitch), _ptr(w_scales),
+                                 _LL(ws), _ptr(out), _LL(out.stride(0)), _DTYPE_CODE[out.dtype], int(add), features, K, 1, None,
+                                 None, 0, 0, _ptr(tc_error_flag(x.device)), _stream()), "gemm_fp8")
+    return out
+
+
+def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+                     tiles: torch.Tensor, n_tiles: torch.Tensor, tile_rows: int) -> torch.Tensor:
+    """Rows in 8 bits, sorted by group, against each group's own weights: ``out[r] = w[g(r)] @ x[r]`` for the rows of every tile
+    (``tiles`` int32 [max, 3] = group, first row, rows, of which at most ``tile_rows``, 1 to 256; ``n_tiles`` int32 [1] on the
+    device; both from ``moe_sort``). ``w`` is [groups, features, K], ``w_scales`` [ceil(K / 512), groups * features, 4]: what
+    ``quantize_fp8`` makes of the groups' rows under one another. ``out`` [rows, features] is bfloat16 or float32; rows that no
+    tile names are left as they are. A tile that names a group or a first row that is not there computes nothing."""
+    x_pitch, xs = _fp8_operand(x, x_scales, "x")
+    if w.dim() != 3 or w.size(0) < 1 or w.size(1) < 1:
+        raise KernelError(f"w must be [groups, features, K], got {tuple(w.shape)}")
+    G, N, K = w.shape
+    if G > 1 and N > 1 and w.stride(0) != N * w.stride(1):
+        raise KernelError(f"w: the groups' rows must lie under one another, got strides {w.stride()}")
+    w_pitch, ws = _fp8_operand(w.flatten(0, 1), w_scales, "w")
+    rows = x.size(0)
+    if x.size(1) != K:
+        raise KernelError(f"x has {x.size(1)} columns, w has {K}")
+    if out.shape != (rows, N) or out.dtype not in _DTYPE_CODE:
+        raise KernelError(f"out is {tuple(out.shape)} {out.dtype}, the product {(rows, N)} in float32 or bfloat16")
+    _row_stride(out, "out")
+    if not 1 <= tile_rows <= 256:
+        raise KernelError(f"tiles of 1 to 256 rows, got {tile_rows}")
+    if tiles.dtype != torch.int32 or tiles.dim() != 2 or tiles.size(1) != 3 or not tiles.is_contiguous():
+        raise KernelError(f"tiles must be contiguous int32 [tiles, 3], got {tiles.dtype} {tuple(tiles.shape)}")
+    if n_tiles.dtype != torch.int32 or n_tiles.numel() != 1:
+        raise KernelError(f"n_tiles must be one int32, got {n_tiles.dtype} {tuple(n_tiles.shape)}")
+    _fp8_on_device(x, x_scales, w, w_scales, out, tiles, n_tiles)
+    _check(_lib().llmrs_gemm_fp8(_ptr(x), _LL(x_pitch), _ptr(x_scales), _LL(xs), rows, _ptr(w), _LL(w_pitch), _ptr(w_scales), _LL(ws),
+                                 _ptr(out), _LL(out.stride(0)), _DTYPE_CODE[out.dtype], 0, N, K, G, _ptr(tiles), _ptr(n_tiles),
+                                 tiles.size(0), tile_rows, _ptr(tc_error_flag(x.device)), _stream()), "gemm_fp8_grouped")
+    return out
