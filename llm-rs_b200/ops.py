@@ -1933,37 +1933,56 @@ def rglru_step(u: torch.Tensor, w: torch.Tensor, r_bias: torch.Tensor, i_bias: t
 # the least integer >= -127 with which the block's largest magnitude is at most 448. Places past a row's last block hold 2^-127.
 FP8, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 FP8_BLOCK = 128         # numbers of a row that share a scale
-_FP8_WORD = 512         # numbers of a row whose scales are one 32-bit word
 
 
-def _fp8_new(rows: int, K: int, device):
-    """Room for rows in 8 bits: (q, scales, bytes between q's rows)."""
-    pitch = (K + 15) // 16 * 16
-    q = torch.empty((rows, pitch), dtype=FP8, device=device)
-    scales = torch.empty((-(-K // _FP8_WORD), rows, 4), dtype=FP8_SCALE, device=device)
-    return (q if pitch == K else q[:, :K]), scales, pitch
+_fp8_entries = {}
 
 
-def _fp8_on_device(*tensors) -> None:
-    """All on the current CUDA device (a kernel is launched on that device's stream)."""
+def _fp8_entry(name: str, n_args: int, floats=(), wide=()):
+    """An entry point with its argument types set (found once): tensors' addresses, sizes and the stream go in as plain integers, which
+    halves the microseconds of a call against an object made for each. ``wide``, ``floats``: arguments that are no int."""
+    fn = _fp8_entries.get(name)
+    if fn is None:
+        fn = getattr(_lib(), name)
+        fn.argtypes = [ctypes.c_float if i in floats else ctypes.c_void_p if i in wide else ctypes.c_int for i in range(n_args)]
+        _fp8_entries[name] = fn
+    return fn
+
+
+def _fp8_new(like: torch.Tensor, rows: int, K: int):
+    """Room for rows in 8 bits on ``like``'s device: (q, scales, bytes between q's rows)."""
+    pitch = (K + 127) & -128 if K >= 128 else (K + 15) & -16      # (rows on 128-byte lines: what a copy of a block of k fetches)
+    q = like.new_empty((rows, pitch), dtype=FP8)
+    return (q if pitch == K else q[:, :K]), like.new_empty(((K + 511) >> 9, rows, 4), dtype=FP8_SCALE), pitch
+
+
+def _fp8_stream(*tensors) -> int:
+    """The current stream of the device that all the tensors are on, which has to be the current device."""
+    at = -1
     for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise KernelError("tensors must be on a CUDA device (this engine has no CPU path)")
-    at = {t.device.index for t in tensors if t is not None}
+        if t is not None:
+            d = t.get_device()
+            if d < 0:
+                raise KernelError("tensors must be on a CUDA device (this engine has no CPU path)")
+            if at >= 0 and d != at:
+                raise KernelError(f"tensors on the devices {at} and {d}")
+            at = d
     current = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-    if at != {current}:
-        raise KernelError(f"tensors on devices {sorted(at)}, the current device is {current}")
+    if at != current:
+        raise KernelError(f"tensors on device {at}, the current device is {current}")
+    return _raw_stream(current) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-def _fp8_rows(x: torch.Tensor, name: str, K: Optional[int] = None) -> int:
+def _fp8_rows(x: torch.Tensor, name: str) -> int:
     """The row stride of a matrix of float32 or bfloat16 with dense rows."""
     if x.dtype not in _DTYPE_CODE:
         raise KernelError(f"{name}: kernels take float32 or bfloat16, not {x.dtype}")
     if x.dim() != 2 or x.size(1) < 1:
         raise KernelError(f"{name} must be [rows, numbers], got {tuple(x.shape)}")
-    if K is not None and x.size(1) != K:
-        raise KernelError(f"{name} has {x.size(1)} columns, expected {K}")
-    return x.size(1) if x.size(0) == 1 else _row_stride(x, name)
+    stride, one = x.stride()
+    if one != 1 and x.size(1) > 1:
+        raise KernelError(f"{name} must have dense rows, got sizes {tuple(x.shape)} strides {x.stride()}")
+    return x.size(1) if x.size(0) == 1 else stride
 
 
 def _fp8_operand(q: torch.Tensor, scales: torch.Tensor, name: str):
@@ -1973,19 +1992,23 @@ def _fp8_operand(q: torch.Tensor, scales: torch.Tensor, name: str):
     if q.dim() != 2 or q.size(1) < 1:
         raise KernelError(f"{name} must be [rows, K], got {tuple(q.shape)}")
     rows, K = q.shape
-    words = -(-K // _FP8_WORD)
+    words = (K + 511) >> 9
     if scales.shape != (words, rows, 4):
         raise KernelError(f"{name} is {tuple(q.shape)}: its scales must be {(words, rows, 4)}, got {tuple(scales.shape)}")
     if rows == 0:
-        return (K + 15) // 16 * 16, 0
-    pitch = q.stride(0) if rows > 1 else (K + 15) // 16 * 16
-    if (K > 1 and q.stride(1) != 1) or pitch % 16 or pitch < K or q.data_ptr() % 16:
+        return (K + 15) & -16, 0
+    pitch, one = q.stride()
+    if rows == 1:
+        pitch = (K + 15) & -16
+    if (K > 1 and one != 1) or pitch % 16 or pitch < K or q.data_ptr() % 16:
         raise KernelError(f"{name}: rows must be dense and start at multiples of 16 bytes, got strides {q.stride()}")
-    stride = scales.stride(0) if words > 1 else 4 * rows
-    if scales.stride(2) != 1 or (rows > 1 and scales.stride(1) != 4) or stride % 4 or stride < 0 or scales.data_ptr() % 4:
+    stride, row, byte = scales.stride()
+    if words == 1:
+        stride = 4 * rows
+    if byte != 1 or (rows > 1 and row != 4) or stride % 4 or stride < 0 or scales.data_ptr() % 4:
         raise KernelError(f"{name}: a word of four scales must be dense, and words of neighbouring rows adjacent, got strides "
                           f"{scales.stride()}")
-    return pitch, stride // 4
+    return pitch, stride >> 2
 
 
 def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
@@ -1997,11 +2020,12 @@ def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
     if src is not None:
         if src.dtype != torch.int32 or src.dim() != 1 or not src.is_contiguous():
             raise KernelError(f"src must be a contiguous int32 vector, got {src.dtype} {tuple(src.shape)}")
-    _fp8_on_device(x, src)
+    stream = _fp8_stream(x, src)
     n = rows if src is None else src.numel()
-    q, scales, pitch = _fp8_new(n, K, x.device)
-    _check(_lib().llmrs_quantize_fp8(_ptr(x), _DTYPE_CODE[x.dtype], _LL(stride), rows, _ptr(src), _ptr(q), _LL(pitch),
-                                     _ptr(scales), n, K, _stream()), "quantize_fp8")
+    q, scales, pitch = _fp8_new(x, n, K)
+    fn = _fp8_entries.get("llmrs_quantize_fp8") or _fp8_entry("llmrs_quantize_fp8", 11, wide=(0, 2, 4, 5, 6, 7, 10))
+    _check(fn(x.data_ptr(), _DTYPE_CODE[x.dtype], stride, rows, None if src is None else src.data_ptr(), q.data_ptr(), pitch,
+              scales.data_ptr(), n, K, stream), "quantize_fp8")
     return q, scales
 
 
@@ -2009,16 +2033,16 @@ def silu_mul_fp8(gate_up: torch.Tensor, block: int = 0, unit=PLAIN_SILU):
     """``silu_mul`` with its result in 8 bits: ``(q, scales)`` of ``silu(gate) * up`` for ``gate_up`` [rows, 2I] that holds gate and
     up in alternating runs of ``block`` columns (0: I gate columns, then I up columns; else a divisor of I). The unit is
     computed in float32 and rounded once."""
-    stride = _fp8_rows(gate_up, "gate_up")
+    stride_in = _fp8_rows(gate_up, "gate_up")
     rows, two = gate_up.shape
     inter = two // 2
     if two % 2 or block < 0 or (block and inter % block):
         raise KernelError(f"gate_up has {two} columns: not two times a multiple of runs of {block}")
-    _fp8_on_device(gate_up)
-    q, scales, pitch = _fp8_new(rows, inter, gate_up.device)
-    _check(_lib().llmrs_silu_mul_fp8(_ptr(gate_up), _DTYPE_CODE[gate_up.dtype], _LL(stride), block or inter,
-                                     *map(ctypes.c_float, unit), _ptr(q), _LL(pitch), _ptr(scales), rows, inter, _stream()),
-           "silu_mul_fp8")
+    stream = _fp8_stream(gate_up)
+    q, scales, pitch = _fp8_new(gate_up, rows, inter)
+    fn = _fp8_entries.get("llmrs_silu_mul_fp8") or _fp8_entry("llmrs_silu_mul_fp8", 13, (4, 5, 6), (0, 2, 7, 8, 9, 12))
+    _check(fn(gate_up.data_ptr(), _DTYPE_CODE[gate_up.dtype], stride_in, block or inter, *unit, q.data_ptr(), pitch,
+              scales.data_ptr(), rows, inter, stream), "silu_mul_fp8")
     return q, scales
 
 
@@ -2038,13 +2062,19 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
         raise KernelError(f"delta {tuple(delta.shape)} ({delta.dtype}) must be float32 or bfloat16 rows like h {tuple(h.shape)}")
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
         raise KernelError(f"rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
-    _fp8_on_device(h, delta, weight, rows)
+    stream = _fp8_stream(h, delta, weight, rows)
     m = n if rows is None else rows.numel()
-    q, scales, pitch = _fp8_new(m, K, h.device)
-    _check(_lib().llmrs_add_rmsnorm_fp8(_ptr(h), _ptr(delta), BF16 if delta is not None and delta.dtype == torch.bfloat16 else F32,
-                                        _ptr(weight), _ptr(rows), n, ctypes.c_float(eps), _ptr(q), _LL(pitch), _ptr(scales), m, K,
-                                        _stream()), "add_rmsnorm_fp8")
+    q, scales, pitch = _fp8_new(h, m, K)
+    fn = _fp8_entries.get("llmrs_add_rmsnorm_fp8") or _fp8_entry("llmrs_add_rmsnorm_fp8", 13, (6,), (0, 1, 3, 4, 7, 8, 9, 12))
+    _check(fn(h.data_ptr(), None if delta is None else delta.data_ptr(), F32 if delta is None else _DTYPE_CODE[delta.dtype],
+              weight.data_ptr(), None if rows is None else rows.data_ptr(), n, eps, q.data_ptr(), pitch, scales.data_ptr(), m, K,
+              stream), "add_rmsnorm_fp8")
     return q, scales
+
+
+def _fp8_product():
+    return _fp8_entries.get("llmrs_gemm_fp8") or _fp8_entry("llmrs_gemm_fp8", 24,
+                                                            wide=(0, 1, 2, 3, 5, 6, 7, 8, 9, 10, 16, 17, 22, 23))
 
 
 def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
@@ -2067,18 +2097,18 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
         raise KernelError("the residual epilogue needs the stream it adds to as out")
     if out is None:
         dtype_code(out_dtype)
-        _fp8_on_device(x, x_scales, w, w_scales)
-        out = torch.empty((tokens, features), dtype=out_dtype, device=x.device)
+        stream = _fp8_stream(x, x_scales, w, w_scales)
+        out = x.new_empty((tokens, features), dtype=out_dtype)
     else:
         if out.dtype != (torch.float32 if add else out_dtype) or out.shape != (tokens, features):
             raise KernelError(f"out is {tuple(out.shape)} {out.dtype}, the product {(tokens, features)} "
                               f"{torch.float32 if add else out_dtype}")
         dtype_code(out.dtype)
         _row_stride(out, "out")
-        _fp8_on_device(x, x_scales, w, w_scales, out)
-    _check(_lib().llmrs_gemm_fp8(_ptr(x), _LL(x_pitch), _ptr(x_scales), _LL(xs), tokens, _ptr(w), _LL(w_pitch), _ptr(w_scales),
-                                 _LL(ws), _ptr(out), _LL(out.stride(0)), _DTYPE_CODE[out.dtype], int(add), features, K, 1, None,
-                                 None, 0, 0, _ptr(tc_error_flag(x.device)), _stream()), "gemm_fp8")
+        stream = _fp8_stream(x, x_scales, w, w_scales, out)
+    _check(_fp8_product()(x.data_ptr(), x_pitch, x_scales.data_ptr(), xs, tokens, w.data_ptr(), w_pitch, w_scales.data_ptr(), ws,
+                          out.data_ptr(), out.stride(0), _DTYPE_CODE[out.dtype], add, features, K, 1, None, None, 0, 0, 0, 0,
+                          tc_error_flag(x.device).data_ptr(), stream), "gemm_fp8")
     return out
 
 
@@ -2108,8 +2138,8 @@ def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
         raise KernelError(f"tiles must be contiguous int32 [tiles, 3], got {tiles.dtype} {tuple(tiles.shape)}")
     if n_tiles.dtype != torch.int32 or n_tiles.numel() != 1:
         raise KernelError(f"n_tiles must be one int32, got {n_tiles.dtype} {tuple(n_tiles.shape)}")
-    _fp8_on_device(x, x_scales, w, w_scales, out, tiles, n_tiles)
-    _check(_lib().llmrs_gemm_fp8(_ptr(x), _LL(x_pitch), _ptr(x_scales), _LL(xs), rows, _ptr(w), _LL(w_pitch), _ptr(w_scales), _LL(ws),
-                                 _ptr(out), _LL(out.stride(0)), _DTYPE_CODE[out.dtype], 0, N, K, G, _ptr(tiles), _ptr(n_tiles),
-                                 tiles.size(0), tile_rows, _ptr(tc_error_flag(x.device)), _stream()), "gemm_fp8_grouped")
+    stream = _fp8_stream(x, x_scales, w, w_scales, out, tiles, n_tiles)
+    _check(_fp8_product()(x.data_ptr(), x_pitch, x_scales.data_ptr(), xs, rows, w.data_ptr(), w_pitch, w_scales.data_ptr(), ws,
+                          out.data_ptr(), out.stride(0), _DTYPE_CODE[out.dtype], 0, N, K, G, tiles.data_ptr(), n_tiles.data_ptr(),
+                          tiles.size(0), tile_rows, 0, 0, tc_error_flag(x.device).data_ptr(), stream), "gemm_fp8_grouped")
     return out
