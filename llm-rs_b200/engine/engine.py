@@ -30,6 +30,9 @@ class EngineConfig:
     page_size: int = 16                  # llm-core/src/backends/candle.rs:827
     dtype: str = "bfloat16"              # "bfloat16" or "float32"
     device: str = "cuda:0"
+    # "stored", or "fp8": attention projections, feed-forwards and experts in 8 bits (bfloat16 engines; the weights are
+    # quantised as they are loaded, the activations in every step).
+    products: str = "stored"
     max_requests: int = 64               # live requests (state slots)
     max_tokens_per_step: int = 2048
     prefill_chunk: int = 512
@@ -47,7 +50,7 @@ class Engine:
         self.runner = runner or ModelRunner.from_model_dir(
             config.model_path, dtype=dtype, device=config.device,
             max_tokens=config.block_pool_size * config.page_size, page_size=config.page_size,
-            max_requests=config.max_requests)
+            max_requests=config.max_requests, products=config.products)
         self.runner.use_graphs = config.cuda_graphs
         self.scheduler = Scheduler(
             self.runner.manager, self.runner.max_positions, self.runner.spec.eos_token_ids,

@@ -102,7 +102,11 @@ class ModelRunner:
     """A model on the device with its cache; owns the step function."""
 
     def __init__(self, spec: ModelSpec, tensors: Dict[str, torch.Tensor], act_dtype: torch.dtype, device,
-                 max_tokens: int, page_size: int = 16, max_requests: int = 64):
+                 max_tokens: int, page_size: int = 16, max_requests: int = 64, products: str = "stored"):
+        if products not in ("stored", "fp8"):
+            raise ValueError(f"products {products!r}: 'stored' or 'fp8'")
+        if products == "fp8" and act_dtype != torch.bfloat16:
+            raise ValueError(f"products in 8 bits come with bfloat16 activations, not {act_dtype}")
         if not torch.cuda.is_available():
             raise StepError("no CUDA device: this engine runs on the GPU only")
         self.device = torch.device(device)
@@ -117,7 +121,7 @@ class ModelRunner:
         # every token bounds it by the pool; a window group gives pages back as it goes, state takes none.
         keeps_all = any(need is not None and need.kind != "window" for need, _ in needs)
         self.max_positions = min(spec.max_positions, n_pages * page_size) if keeps_all else spec.max_positions
-        self.model.bind(tensors, Runtime(self.device, act_dtype, self.max_positions))
+        self.model.bind(tensors, Runtime(self.device, act_dtype, self.max_positions, products))
         self.storage = CacheStorage(needs, spec.run_order, page_size, n_pages, max_requests, act_dtype, self.device)
         self.manager = CacheManager(self.storage.groups, page_size, max_requests)
         self._scratch_bufs: Dict[str, torch.Tensor] = {}

@@ -2112,6 +2112,14 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     return out
 
 
+def fp8_tile_rows(n_rows: int, n_groups: int) -> int:
+    """Rows per tile for ``moe_sort`` and ``gemm_fp8_grouped``, by the rows a group has on average: a tile's rows reserve shared
+    memory, so that larger tiles leave fewer of the weights' copies under way; smaller ones read a group's weights again. One
+    product, us (32 groups of 2,048 x 2,048), tiles of 32 | 64 | 128 | 256 rows by rows a group: 4 22 | 24 | 24 | 27; 16 25 | 26 | 27 |
+    34; 32 29 | 27 | 28 | 30; 64 41 | 33 | 31 | 37; 128 61 | 48 | 39 | 43; 256 109 | 75 | 60 | 52."""
+    return 32 if n_rows <= 16 * n_groups else 64 if n_rows <= 48 * n_groups else 128 if n_rows <= 160 * n_groups else 256
+
+
 def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
                      tiles: torch.Tensor, n_tiles: torch.Tensor, tile_rows: int) -> torch.Tensor:
     """Rows in 8 bits, sorted by group, against each group's own weights: ``out[r] = w[g(r)] @ x[r]`` for the rows of every tile

@@ -11,7 +11,7 @@ import numpy as np
 
 from .. import host, ops
 from .base import Mixer, Plan, PositionEncoding, PreNormed, Runtime, StepInfo
-from .linear import Linear
+from .linear import Fp8Linear, Linear, product_of
 from .registry import build, register
 from .spec import CacheNeed, PartSpec, WeightSpec
 
@@ -211,12 +211,14 @@ class GQAttention(Mixer):
         bqkv = None
         if self.bias:
             bqkv = torch.cat([tensors[nm(r, "bias")].to(dt) for r in "qkv"], dim=0).contiguous()
-        self.qkv_proj = Linear(wqkv, bqkv, runtime.act_dtype)
+        self.qkv_proj = product_of(wqkv, bqkv, runtime)
         self.qkv_proj.warms_next = False
         # The query rows alone, for run-order entries that read another entry's cache.
-        self.q_proj = Linear(wqkv[: self.q_width], None if bqkv is None else bqkv[: self.q_width], runtime.act_dtype)
+        self.takes_rows8 = isinstance(self.qkv_proj, Fp8Linear)
+        self.q_proj = (self.qkv_proj.rows(self.q_width) if self.takes_rows8 else
+                       Linear(wqkv[: self.q_width], None if bqkv is None else bqkv[: self.q_width], runtime.act_dtype))
         self.qkv_proj.tc_max_tokens = self.q_proj.tc_max_tokens = QKV_TC_MAX_TOKENS
-        self.o_proj = Linear(tensors[nm("o")], tensors.get(nm("o", "bias")), runtime.act_dtype)
+        self.o_proj = product_of(tensors[nm("o")], tensors.get(nm("o", "bias")), runtime)
         self.q_norm_w = self.k_norm_w = None
         if self.qk_norm:
             self.q_norm_w = tensors[nm("q_norm")].to(torch.float32).contiguous()

@@ -26,6 +26,13 @@ class Runtime:
     device: torch.device
     act_dtype: torch.dtype          # bfloat16 or float32: type of activations and of the cache
     max_positions: int              # positions 0 .. max_positions-1 can occur
+    # "stored": products of the weights as they are; "fp8": the attention projections, the feed-forward's and the experts'
+    # products of bfloat16 weights in 8 bits (``parts.linear.Fp8Linear``). Everything else stays as it is stored.
+    products: str = "stored"
+
+    @property
+    def fp8(self) -> bool:
+        return self.products == "fp8"
 
 
 @dataclass
@@ -100,6 +107,19 @@ class PreNormed:
         return (self.parts, self.n_parts, self.dim, self.eps)
 
 
+class Rows8:
+    """Rows in 8 bits (``ops.quantize_fp8``) on their way to an ``Fp8Linear``: a part whose ``takes_rows8`` is true gets this
+    object as its ``x`` from a norm that made it (``Norm.rows8``) instead of rows in the activation type."""
+    __slots__ = ("q", "scales")
+    dtype = None        # neither of the activation types
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor):
+        self.q, self.scales = q, scales
+
+    def size(self, dim: int) -> int:
+        return self.q.size(dim)
+
+
 class Norm(Part):
     """``forward(h, delta)``: ``h += delta`` (float32 residual stream, in place; ``delta``
     may be None) and return the normed rows in the activation type. With ``rows`` only
@@ -111,6 +131,11 @@ class Norm(Part):
     def link(self):
         """(weight float32 [dim], eps) when this norm is ``x / sqrt(mean(x^2) + eps) * weight`` and may be
         spread over the products around it (see ``PreNormed``); None otherwise."""
+        return None
+
+
+    def rows8(self, h: torch.Tensor, delta: Optional[torch.Tensor]) -> Optional["Rows8"]:
+        """``forward`` with its result in 8 bits, or None where this norm cannot."""
         return None
 
 
@@ -144,6 +169,7 @@ class Mixer(Part):
     stream) and may add its output into it itself, returning None.
     """
     fuses_residual = False
+    takes_rows8 = False         # ``forward`` accepts ``Rows8`` as ``x`` (set by ``bind``)
 
     def takes_prenormed(self, n_tokens: int) -> bool:
         """True when ``forward`` accepts a ``PreNormed`` as ``x`` in a step of ``n_tokens`` tokens."""
@@ -179,6 +205,7 @@ class FeedForward(Part):
     """``forward(x, ctx)``: [tokens, hidden] -> [tokens, hidden], token by token. With
     ``fuses_residual = True`` it also takes ``residual=h`` as a mixer does."""
     fuses_residual = False
+    takes_rows8 = False
 
     def takes_prenormed(self, n_tokens: int) -> bool:
         return False

@@ -59,10 +59,16 @@ class PreNormBlock(Block):
     def accepts_prenormed(self, n_tokens: int) -> bool:
         return LINK_NORMS and self.mixer_norm.link() is not None and self.mixer.takes_prenormed(n_tokens)
 
+    @staticmethod
+    def _normed(norm, part, h, delta):
+        """The norm's rows for ``part``: in 8 bits where it takes them."""
+        x = norm.rows8(h, delta) if getattr(part, "takes_rows8", False) else None
+        return norm.forward(h, delta) if x is None else x
+
     def forward(self, h, pending, ctx, cache, next_norm=None):
         n = ctx.n_tokens
         # A PreNormed ``pending`` was made for this block's first norm by the block before (h holds the sum).
-        x = pending if isinstance(pending, PreNormed) else self.mixer_norm.forward(h, pending)
+        x = pending if isinstance(pending, PreNormed) else self._normed(self.mixer_norm, self.mixer, h, pending)
         fused = getattr(self.mixer, "fuses_residual", False)
         if self.feed_forward is None:
             if next_norm is not None and fused and self.mixer.emits_prenormed(n):
@@ -73,7 +79,7 @@ class PreNormBlock(Block):
             y = self.mixer.forward(x, ctx, cache, residual=h, next_norm=link)
         else:
             a = self.mixer.forward(x, ctx, cache, residual=h) if fused else self.mixer.forward(x, ctx, cache)
-            y = self.feed_forward_norm.forward(h, a)
+            y = self._normed(self.feed_forward_norm, self.feed_forward, h, a)
         fused = getattr(self.feed_forward, "fuses_residual", False)
         if next_norm is not None and fused and self.feed_forward.emits_prenormed(n):
             return h, self.feed_forward.forward(y, ctx, residual=h, next_norm=next_norm)

@@ -11,7 +11,8 @@ epilogue (``parts/mlp.py``), which runs this package's kernel for many tokens (t
 sends every product of steps of n tokens or more to that kernel, with the residual sum and the
 norms spread over its epilogues as in decode steps. float32 weights, the whole float32 path and
 tensors that the model folder stores in 32-bit, go through this package's own FFMA
-kernel: true 32-bit, no reduced-precision tensor-core mode.
+kernel: true 32-bit, no reduced-precision tensor-core mode. With ``Runtime.products`` "fp8" the parts that ask for it
+(``product_of``) run bfloat16 weights in 8 bits (``Fp8Linear``).
 """
 from __future__ import annotations
 
@@ -21,7 +22,7 @@ from typing import Optional
 import torch
 
 from .. import ops
-from .base import PreNormed
+from .base import PreNormed, Rows8, Runtime
 
 # Steps with at most this many tokens take the tcgen05 kernel for few tokens; 0 switches the tcgen05 products off.
 # (Measured inside decode steps at Qwen3-8B sizes: with its fused epilogues the kernel is ahead of the library product
@@ -145,3 +146,43 @@ class Linear:
             ops.gemm_bf16(x, self.weight, out=h, epilogue="residual", then=self.next_weight)
             return None
         return self.forward(x)
+
+
+class Fp8Linear(Linear):
+    """``y = x @ weight.T`` with ``x`` and ``weight`` in 8 bits (e4m3 with a power of two for each block of 128 numbers along
+    k, see ``ops.quantize_fp8``): the weights are quantised once, when the part is bound; the rows of ``x`` in every step, by
+    the kernel that makes them (a norm, a gated unit: ``Rows8``) or by one of their own. Sums are float32. No epilogue but the sum
+    into the residual stream; no norms spread over the products."""
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, act_dtype: torch.dtype):
+        self.weight, self.scales, self.bias, self.act_dtype = weight, scales, None, act_dtype
+        self.next_weight, self.warms_next, self.tc_max_tokens, self.tc_ok = None, False, None, False
+
+    @classmethod
+    def of(cls, weight: torch.Tensor, act_dtype: torch.dtype) -> "Fp8Linear":
+        return cls(*ops.quantize_fp8(weight), act_dtype)
+
+    def rows(self, n: int) -> "Fp8Linear":
+        """The product of the first ``n`` rows of the weight (shared, not copied)."""
+        return Fp8Linear(self.weight[:n], self.scales[:, :n], self.act_dtype)
+
+    @staticmethod
+    def _rows8(x):
+        return (x.q, x.scales) if isinstance(x, Rows8) else ops.quantize_fp8(x)
+
+    def forward(self, x, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return ops.gemm_fp8(*self._rows8(x), self.weight, self.scales, out_dtype=out_dtype or self.act_dtype)
+
+    def forward_into_residual(self, x, h: torch.Tensor) -> Optional[torch.Tensor]:
+        if not h.is_contiguous():
+            return self.forward(x)
+        ops.gemm_fp8(*self._rows8(x), self.weight, self.scales, out=h, epilogue="residual")
+        return None
+
+
+def product_of(weight: torch.Tensor, bias: Optional[torch.Tensor], runtime: Runtime) -> Linear:
+    """The product of a part that may run in 8 bits: with ``Runtime.products`` "fp8" an ``Fp8Linear`` of a bfloat16 weight without
+    a bias, else a ``Linear``."""
+    if runtime.fp8 and bias is None and weight.dtype == torch.bfloat16:
+        return Fp8Linear.of(weight, runtime.act_dtype)
+    return Linear(weight, bias, runtime.act_dtype)

@@ -7,8 +7,8 @@ from typing import Optional
 import torch
 
 from .. import ops
-from .base import FeedForward, PreNormed, Runtime
-from .linear import Linear
+from .base import FeedForward, PreNormed, Rows8, Runtime
+from .linear import Fp8Linear, Linear, product_of
 from .registry import register
 from .spec import WeightSpec
 
@@ -59,8 +59,9 @@ class SwiGLU(FeedForward):
             w = ops.interleave_gate_up(g.to(dt), u.to(dt))
         else:
             w = torch.cat([g.to(dt), u.to(dt)], dim=0).contiguous()
-        self.gate_up = Linear(w, None, runtime.act_dtype)
-        self.down = Linear(tensors[self._name("down")], None, runtime.act_dtype)
+        self.gate_up = product_of(w, None, runtime)
+        self.down = product_of(tensors[self._name("down")], None, runtime)
+        self.takes_rows8 = isinstance(self.gate_up, Fp8Linear)
 
     def chain(self):
         return [self.gate_up, self.down]
@@ -85,6 +86,8 @@ class SwiGLU(FeedForward):
         # 64 tokens), for many the persistent tcgen05 kernel on pairs of SMs (2,048 tokens: 261 against 271 + 20 us).
         if self.block and x.dtype == torch.bfloat16 and self.gate_up.tc_enabled() and FUSE_GATE_UP:
             act = ops.gemm_bf16(x, self.gate_up.weight, epilogue="silu_mul", then=self.gate_up.next_weight, unit=self.unit)
+        elif isinstance(self.down, Fp8Linear):      # the unit's result goes into the next product in 8 bits
+            act = Rows8(*ops.silu_mul_fp8(self.gate_up.forward(x), block=self.block, unit=self.unit))
         else:
             act = ops.silu_mul(self.gate_up.forward(x), block=self.block, unit=self.unit)
         if next_norm is not None:
@@ -127,8 +130,9 @@ class DenseFF(FeedForward):
         return specs
 
     def bind(self, tensors, runtime: Runtime):
-        self.up = Linear(tensors[self.prefix + self.names["up"]], None, runtime.act_dtype)
-        self.down = Linear(tensors[self.prefix + self.names["down"]], None, runtime.act_dtype)
+        self.up = product_of(tensors[self.prefix + self.names["up"]], None, runtime)
+        self.down = product_of(tensors[self.prefix + self.names["down"]], None, runtime)
+        self.takes_rows8 = isinstance(self.up, Fp8Linear)
         if self.activation == "polynorm":
             self.coeff = tensors[self.prefix + self.names["act"]].to(torch.float32).contiguous()
         elif self.activation == "xielu":      # the two branches' factors, made once in double

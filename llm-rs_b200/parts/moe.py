@@ -41,7 +41,8 @@ class MixtureOfExperts(FeedForward):
     ``sigmoid(w_sg . x)``, one number per token, computed beside the router's logits.
 
     The rows are sorted by expert so that a tile of rows shares one expert's weights; the first product has the gated
-    unit as its epilogue; bfloat16 products run on the tensor cores (``csrc/gemm_grouped.cu``). ``forward`` takes the
+    unit as its epilogue; bfloat16 products run on the tensor cores (``csrc/gemm_grouped.cu``). With ``Runtime.products`` "fp8"
+    both products run in 8 bits (``csrc/gemm_fp8.cu``), the unit between them a kernel whose result is in 8 bits. ``forward`` takes the
     float32 residual stream itself (``reads_residual``) and rounds its rows to the activation type. Tensor names: ``<prefix>e<i>.gate|up|down`` and
     ``<prefix>table`` unless ``names`` renames the roles."""
 
@@ -116,7 +117,17 @@ class MixtureOfExperts(FeedForward):
         self.act_dtype = runtime.act_dtype
         stack = lambda role: torch.stack([tensors[self._name(e, role)] for e in range(self.n_experts)]).contiguous()
         self.w_gate, self.w_up, self.w_down = stack("gate"), stack("up"), stack("down")
-        if len({self.w_gate.dtype, self.w_up.dtype, self.w_down.dtype}) != 1:
+        self.fp8 = None
+        if runtime.fp8 and {self.w_gate.dtype, self.w_up.dtype, self.w_down.dtype} == {torch.bfloat16}:
+            # Gate and up are one product, their rows alternating by 64 where that divides, as the dense feed-forward's.
+            E, F, H = self.w_gate.shape
+            self.block = 64 if F % 64 == 0 else F
+            gate_up = torch.stack([self.w_gate.reshape(-1, self.block, H), self.w_up.reshape(-1, self.block, H)], dim=1)
+            q, scales = ops.quantize_fp8(gate_up.reshape(E * 2 * F, H))
+            q_down, down_scales = ops.quantize_fp8(self.w_down.reshape(E * H, F))
+            self.fp8 = (q.unflatten(0, (E, 2 * F)), scales, q_down.unflatten(0, (E, H)), down_scales)
+            self.w_gate = self.w_up = self.w_down = None
+        elif len({self.w_gate.dtype, self.w_up.dtype, self.w_down.dtype}) != 1:
             self.w_gate, self.w_up, self.w_down = (w.to(torch.float32) for w in (self.w_gate, self.w_up, self.w_down))
         self.table = self.router_w = self.router_w_stored = self.router_b = self.shared = None
         if self.router == "table":
@@ -172,7 +183,8 @@ class MixtureOfExperts(FeedForward):
             expert_of, weight_of = ops.moe_route_biased(logits, self.correction, self.n_experts + self.n_identity,
                                                         self.n_experts, self.top)
         n_rows = expert_of.numel()
-        tile_rows = ops.grouped_tile_rows(n_rows, self.n_experts, self.w_gate.numel())
+        tile_rows = (ops.fp8_tile_rows(n_rows, self.n_experts) if self.fp8 else
+                     ops.grouped_tile_rows(n_rows, self.n_experts, self.w_gate.numel()))
         if self.n_identity:
             # Assignments to identity experts are sorted into one more group that runs no product; the weighted sum
             # takes the token's own row for them.
@@ -180,11 +192,18 @@ class MixtureOfExperts(FeedForward):
                                                              tiled_groups=self.n_experts)
         else:
             row_of, src_token, tiles, n_tiles = ops.moe_sort(expert_of, self.top, self.n_experts, tile_rows)
-        act = torch.empty((n_rows, self.expert_size), dtype=self.act_dtype, device=x.device)
-        ops.gemm_grouped(x, self.w_gate, act, tiles, n_tiles, src_token, w2=self.w_up, limit=self.limit,
-                         alpha=self.alpha, shift=self.up_shift, tile_rows=tile_rows)
         rows = torch.empty((n_rows, self.hidden_size), dtype=torch.float32, device=x.device)
-        ops.gemm_grouped(act, self.w_down, rows, tiles, n_tiles, None, tile_rows=tile_rows)
+        if self.fp8:
+            w, scales, w_down, down_scales = self.fp8
+            gate_up = torch.empty((n_rows, w.size(1)), dtype=self.act_dtype, device=x.device)
+            ops.gemm_fp8_grouped(*ops.quantize_fp8(x, src_token), w, scales, gate_up, tiles, n_tiles, tile_rows)
+            act8 = ops.silu_mul_fp8(gate_up, block=self.block, unit=(self.limit, self.alpha, self.up_shift))
+            ops.gemm_fp8_grouped(*act8, w_down, down_scales, rows, tiles, n_tiles, tile_rows)
+        else:
+            act = torch.empty((n_rows, self.expert_size), dtype=self.act_dtype, device=x.device)
+            ops.gemm_grouped(x, self.w_gate, act, tiles, n_tiles, src_token, w2=self.w_up, limit=self.limit,
+                             alpha=self.alpha, shift=self.up_shift, tile_rows=tile_rows)
+            ops.gemm_grouped(act, self.w_down, rows, tiles, n_tiles, None, tile_rows=tile_rows)
         if self.n_identity:
             y = ops.moe_combine_identity(rows, row_of, weight_of, expert_of, x, self.top, self.n_experts)
             if residual is None:

@@ -6,7 +6,7 @@ from typing import Optional
 import torch
 
 from .. import ops
-from .base import Norm, Runtime
+from .base import Norm, Rows8, Runtime
 from .registry import register
 from .spec import WeightSpec
 
@@ -48,6 +48,11 @@ class RMSNorm(Norm):
         if isinstance(delta, tuple):      # two branch outputs of a block that runs its branches side by side
             return ops.add_two_rmsnorm(h, *delta, self.weight, None, self.eps, self.act_dtype, rows=rows)[0]
         return ops.add_rmsnorm(h, delta, self.weight, self.eps, self.act_dtype, rows=rows)
+
+    def rows8(self, h, delta):
+        if isinstance(delta, tuple):
+            return None
+        return Rows8(*ops.add_rmsnorm_fp8(h, delta, self.weight, self.eps))
 
     def add_normed(self, h, y):
         return ops.outnorm_add(h, y, self.weight, self.eps)

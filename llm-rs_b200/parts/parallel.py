@@ -56,8 +56,8 @@ class ParallelMixer(Mixer):
             side.bind(tensors, runtime)
         self.fused = None
         lo, ro = getattr(self.left, "o_proj", None), getattr(self.right, "o_proj", None)
-        if (FUSE_PARALLEL and all(hasattr(side, "heads") for side in self.sides()) and isinstance(lo, Linear)
-                and isinstance(ro, Linear) and lo.bias is None and ro.bias is None and lo.weight.dtype == ro.weight.dtype):
+        if (FUSE_PARALLEL and all(hasattr(side, "heads") for side in self.sides()) and type(lo) is Linear
+                and type(ro) is Linear and lo.bias is None and ro.bias is None and lo.weight.dtype == ro.weight.dtype):
             self.widths = (lo.weight.size(1), ro.weight.size(1))
             self.fused = Linear(torch.cat([lo.weight, ro.weight], dim=1).contiguous(), None, runtime.act_dtype)
 

@@ -10,7 +10,7 @@ import torch
 from .. import host, ops
 from .attention import _ATTN_TC, PREFILL_TILE, PrefillWork, prefill_kernel
 from .base import Mixer, Plan, Runtime, StepInfo
-from .linear import Linear
+from .linear import product_of
 from .position import wavelength_scaled_frequencies
 from .registry import register
 from .spec import CacheNeed, WeightSpec
@@ -155,12 +155,12 @@ class ScoredAttention(Mixer):
             ws += [g, g.new_zeros((fill, g.size(1)))] if fill else [g]
         dt = ws[0].dtype if all(w.dtype == ws[0].dtype for w in ws) else torch.float32
         wqkv = torch.cat([w.to(dt) for w in ws], dim=0).contiguous()
-        self.qkv_proj = Linear(wqkv, None, runtime.act_dtype)
+        self.qkv_proj = product_of(wqkv, None, runtime)
         # For entries that read another's pages: the queries (and the gates) alone.
         wq = wqkv[: self.q_width] if not self.gated else torch.cat(
             [wqkv[: self.q_width], wqkv[self.q_width + self.k_width + self.v_width:]], dim=0).contiguous()
-        self.q_proj = Linear(wq, None, runtime.act_dtype)
-        self.o_proj = Linear(tensors[nm("o")], None, runtime.act_dtype)
+        self.q_proj = product_of(wq, None, runtime)
+        self.o_proj = product_of(tensors[nm("o")], None, runtime)
         f32 = lambda role: tensors[nm(role)].to(torch.float32).contiguous()
         self.q_norm_w = f32("q_norm") if self.qk_norm in ("whole", "head") else None
         self.k_norm_w = f32("k_norm") if self.qk_norm in ("whole", "head") else None

@@ -203,7 +203,19 @@ def _cost_rglru_step(u, w, r_bias, i_bias, rate, y, y_bias, state, ctx):
     return (f"{u.size(0)} requests, {w.size(0)}x{n}x{n}", _nbytes(w, u, u, u) + u.numel() * 8, 4.0 * u.numel() * n)
 
 
+def _cost_fp8(x, x_scales, w, w_scales, out=None, epilogue="store", out_dtype=torch.bfloat16):
+    tokens, (n, K) = x.size(0), w.shape
+    return (f"{n}x{K}", (tokens + n) * K + _nbytes(x_scales, w_scales) + tokens * n * (8 if epilogue == "residual" else out_dtype.itemsize),
+            2.0 * tokens * n * K)
+
+
+def _cost_fp8_grouped(x, x_scales, w, w_scales, out, *a, **k):
+    return _cost_grouped(x, w, out, None, None, None)
+
+
 WRAPPED: Dict[str, Callable] = {
+    "gemm_fp8": _cost_fp8, "gemm_fp8_grouped": _cost_fp8_grouped, "quantize_fp8": _cost_rows(0), "silu_mul_fp8": _cost_rows(0),
+    "add_rmsnorm_fp8": _cost_rows(0),
     "add_two_rmsnorm": _cost_two_norms, "rglru_gates": _cost_gates, "rglru_step": _cost_rglru_step,
     "rglru_scan": lambda ab, y, y_bias, state, ctx: (f"{ab.size(0)} tokens", _nbytes(ab) + ab.size(0) * ab.size(1) * 2 * y.element_size()
                                                      + 2 * ctx.n_requests * ab.size(1) * 4, 0.0),
