@@ -25,10 +25,14 @@ __device__ __forceinline__ uint32_t f8_scale_byte(float top) {
 // 2^-E of a scale byte up to 247: exact, and a normal number.
 __device__ __forceinline__ float f8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// Two numbers, already divided by their scale, as e4m3 (the lower byte is the first).
+// Two numbers, already divided by their scale, as e4m3 (the lower byte is the first). An infinity would become 448: a block whose
+// maximum is one goes through f8_pack2_any.
 __device__ __forceinline__ uint32_t f8_pack2(float a, float b) {
-  uint32_t r = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  if (isinf(a)) r |= 0x7fu;      // the conversion would make 448 of it
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+static __device__ __noinline__ uint32_t f8_pack2_any(float a, float b) {
+  uint32_t r = f8_pack2(a, b);
+  if (isinf(a)) r |= 0x7fu;
   if (isinf(b)) r |= 0x7f00u;
   return r;
 }

@@ -4,8 +4,9 @@
 // A warp makes 512 numbers of a row, which is one word of scales. Two ways of dealing the numbers to lanes:
 //   rows that start on 32-byte boundaries   a lane takes 16 consecutive numbers (loads of 32 bytes, a store of 16); a block's
 //                                           maximum is the maximum over 8 neighbouring lanes
-//   all others                              a lane takes number lane, lane + 32, .. (loads and stores of one number, coalesced
-//                                           over the warp); a block's maximum is the maximum over the warp
+//   all others                              a lane takes 4 consecutive numbers of each of the four blocks (loads of what is
+//                                           aligned, stores of 4 bytes: q's rows start at multiples of 16); a block's maximum is the
+//                                           maximum over the warp
 #include "fp8.cuh"
 
 constexpr int F8_THREADS = 256;
@@ -49,6 +50,19 @@ __device__ __forceinline__ void f8_store_runs(float (&v)[16], uint8_t* q, uint32
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       p[i] = f8_pack2(v[4 * i] * inv, v[4 * i + 1] * inv) | f8_pack2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16;
+    if (isinf(top)) {
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        float a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = i == 0 ? v[e] : i == 1 ? v[4 + e] : i == 2 ? v[8 + e] : v[12 + e];
+        const uint32_t q4 = f8_pack2_any(a[0] * inv, a[1] * inv) | f8_pack2_any(a[2] * inv, a[3] * inv) << 16;
+        if (i == 0) p[0] = q4;
+        if (i == 1) p[1] = q4;
+        if (i == 2) p[2] = q4;
+        if (i == 3) p[3] = q4;
+      }
+    }
     *reinterpret_cast<uint4*>(q) = make_uint4(p[0], p[1], p[2], p[3]);
   }
   // Lanes 0, 8, 16, 24 hold the four blocks' bytes.
@@ -58,23 +72,43 @@ __device__ __forceinline__ void f8_store_runs(float (&v)[16], uint8_t* q, uint32
   if ((threadIdx.x & 31) == 0) *word = w;
 }
 
-// The warp's 512 numbers dealt by 32 (v[i] is number lane + 32 i); `left` numbers of the row are left.
-__device__ __forceinline__ void f8_store_dealt(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
+// Four consecutive numbers, of which `n` are there (zeros behind them), from any address. bfloat16 numbers come by the words that hold
+// them: a word's other half lies in the same aligned four bytes as the number that is asked for.
+__device__ __forceinline__ void f8_load4(const float* p, int n, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+}
+__device__ __forceinline__ void f8_load4(const __nv_bfloat16* p, int n, float* v) {
+  const uint32_t odd = (uint32_t)((uintptr_t)p >> 1) & 1u;      // the first number is a word's upper half
+  const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)p & ~(uintptr_t)3);
+  if (n >= 4) {
+    const uint32_t a = w[0], b = w[1], c = odd ? w[2] : 0u;
+    const uint32_t lo = __funnelshift_r(a, b, 16 * odd), hi = __funnelshift_r(b, c, 16 * odd);
+    v[0] = __uint_as_float(lo << 16), v[1] = __uint_as_float(lo & 0xffff0000u);
+    v[2] = __uint_as_float(hi << 16), v[3] = __uint_as_float(hi & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+  }
+}
+
+// The warp's 512 numbers by fours (v[4 j + i] is number 128 j + 4 lane + i); `left` numbers of the row are left. The last word of
+// a row of q is written whole.
+__device__ __forceinline__ void f8_store_fours(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
   const int lane = threadIdx.x & 31;
   uint32_t w = 0;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    float top = fmaxf(fmaxf(fabsf(v[4 * b]), fabsf(v[4 * b + 1])), fmaxf(fabsf(v[4 * b + 2]), fabsf(v[4 * b + 3])));
-    top = warp_max(top);
+  for (int j = 0; j < 4; ++j) {
+    // The bits of magnitudes are ordered as whole numbers, whose maximum over a warp is one instruction (a NaN counts as 0).
+    const float own = fmaxf(fmaxf(fmaxf(fabsf(v[4 * j]), fabsf(v[4 * j + 1])), fmaxf(fabsf(v[4 * j + 2]), fabsf(v[4 * j + 3]))), 0.f);
+    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(own)));
     const uint32_t byte = f8_scale_byte(top);
     const float inv = f8_inverse(byte);
-    w |= byte << (8 * b);
-#pragma unroll
-    for (int i = 4 * b; i < 4 * b + 4; i += 2) {
-      const uint32_t two = f8_pack2(v[i] * inv, v[i + 1] * inv);
-      if (lane + 32 * i < left) q[lane + 32 * i] = (uint8_t)two;
-      if (lane + 32 * (i + 1) < left) q[lane + 32 * (i + 1)] = (uint8_t)(two >> 8);
-    }
+    w |= byte << (8 * j);
+    uint32_t p = f8_pack2(v[4 * j] * inv, v[4 * j + 1] * inv) | f8_pack2(v[4 * j + 2] * inv, v[4 * j + 3] * inv) << 16;
+    if (isinf(top))
+      p = f8_pack2_any(v[4 * j] * inv, v[4 * j + 1] * inv) | f8_pack2_any(v[4 * j + 2] * inv, v[4 * j + 3] * inv) << 16;
+    if (128 * j + 4 * lane < left) *reinterpret_cast<uint32_t*>(q + 128 * j + 4 * lane) = p;
   }
   if (lane == 0) *word = w;
 }
@@ -87,38 +121,68 @@ struct F8Rows {
 };
 
 // ---- rows as they are ---------------------------------------------------------------------------------------------
-// Row r from row src[r] (or r) of x; a row whose source is none of x's becomes zeros.
+// Row r from row src[r] (or r) of x; a row whose source is none of x's becomes zeros. A warp makes two words of a row, so that
+// the loads of both are in flight (7,211 rows of 4,096 bfloat16 numbers: 16.1 us with one, 15.0 with two; 13.8 at 6.45 TB/s).
 template <typename T, bool RUNS>
 __global__ void __launch_bounds__(F8_THREADS)
 f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, const int* __restrict__ src, const F8Rows o) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int r = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5), word = blockIdx.y;      // a block: one word of eight rows
+  const int r = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5);      // a block: two words of eight rows
   if (r >= o.rows) return;
-  const int from = src ? src[r] : r, at = word * F8_WORD, left = o.width - at;
+  const int from = src ? src[r] : r;
   const bool live = from >= 0 && from < x_rows;
-  const T* xr = x + (live ? (size_t)from * x_stride : 0) + at;
-  uint8_t* q = o.q + (size_t)r * o.pitch + at;
-  uint32_t* w = o.words + (size_t)word * o.rows + r;
-  float v[16];
+  const T* xr = x + (live ? (size_t)from * x_stride : 0);
+  float v[2][16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  if (RUNS) {
-    if (live && 16 * lane < left) f8_load16(xr + 16 * lane, v);
-    f8_store_runs(v, 16 * lane < left ? q + 16 * lane : nullptr, w);
-  } else {
+  for (int h = 0; h < 2; ++h) {
+    const int at = (2 * blockIdx.y + h) * F8_WORD, left = live ? o.width - at : 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (live && lane + 32 * i < left) v[i] = to_float(xr[lane + 32 * i]);
-    f8_store_dealt(v, q, left, w);
+    for (int i = 0; i < 16; ++i) v[h][i] = 0.f;
+    if (RUNS) {
+      if (16 * lane < left) f8_load16(xr + at + 16 * lane, v[h]);
+    } else if (left >= F8_WORD) {      // no branch between the loads: they are in flight together
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f8_load4(xr + at + 128 * j + 4 * lane, 4, v[h] + 4 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (128 * j + 4 * lane < left) f8_load4(xr + at + 128 * j + 4 * lane, left - 128 * j - 4 * lane, v[h] + 4 * j);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int word = 2 * blockIdx.y + h, left = o.width - word * F8_WORD;
+    if (left <= 0) break;
+    uint8_t* q = o.q + (size_t)r * o.pitch + word * F8_WORD;
+    uint32_t* w = o.words + (size_t)word * o.rows + r;
+    if (RUNS)
+      f8_store_runs(v[h], 16 * lane < left ? q + 16 * lane : nullptr, w);
+    else
+      f8_store_fours(v[h], q, left, w);
   }
 }
 
 // ---- the gated unit -------------------------------------------------------------------------------------------------
-template <typename T, bool RUNS>
+// GatedUnit in fewer instructions: the quotient by an approximate reciprocal and one step of the remainder, off by less than an ulp as
+// a division is; PLAIN is silu(gate) * up. What bounds the kernel is these instructions beside the memory: 2,048 rows of 12,288
+// took 33 us with the division, 24.5 with this (19.5 at 6.45 TB/s).
+template <bool PLAIN>
+__device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, float up) {
+  const float g = PLAIN ? gate : fminf(gate, unit.limit), u = PLAIN ? up : fminf(fmaxf(up, -unit.limit), unit.limit);
+  const float d = 1.0f + expf(PLAIN ? -g : -unit.alpha * g);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));      // (0 from 2^126 on: the unit of a gate below -87 is 0)
+  const float q = g * r, better = fmaf(fmaf(-q, d, g), r, q);
+  return (d < INFINITY ? better : q) * (PLAIN ? u : u + unit.shift);
+}
+
+// `shift`: block = 2^shift, or -1. WAY 0: runs of 16 columns that start on 32-byte boundaries and lie within a run of `block`; 1: fours that do (or the plain
+// layout, block = width); 2: any.
+template <typename T, int WAY, bool PLAIN>
 __global__ void __launch_bounds__(F8_THREADS)
-f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, const GatedUnit unit, const F8Rows o) {
+f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shift, const GatedUnit unit, const F8Rows o) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -128,31 +192,63 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, const G
   const T* row = gu + (size_t)r * gu_stride;
   uint8_t* q = o.q + (size_t)r * o.pitch + at;
   uint32_t* w = o.words + (size_t)word * o.rows + r;
+  const bool whole = block == o.width;
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  if (RUNS) {      // a run of 16 columns lies within a run of `block`
+  if (WAY == 0) {
     const int c = at + 16 * lane;
     if (16 * lane < left) {
       float g[16];
-      const T* p = row + (size_t)(c / block) * 2 * block + c % block;
+      const T* p = row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block);
       f8_load16(p, g);
       f8_load16(p + block, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = unit(g[i], v[i]);
+      for (int i = 0; i < 16; ++i) v[i] = f8_unit<PLAIN>(unit, g[i], v[i]);
     }
     f8_store_runs(v, 16 * lane < left ? q + 16 * lane : nullptr, w);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int c = at + lane + 32 * i;
-      if (c < o.width) {
-        const T* p = row + (size_t)(c / block) * 2 * block + c % block;
-        v[i] = unit(to_float(p[0]), to_float(p[block]));
-      }
-    }
-    f8_store_dealt(v, q, left, w);
+    return;
   }
+  float g[16];
+  if (WAY == 1 && left >= F8_WORD) {      // no branch between the loads: they are in flight together
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = at + 128 * j + 4 * lane;
+      const T* p = row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block);
+      f8_load4(p, 4, g + 4 * j);
+      f8_load4(p + block, 4, v + 4 * j);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = f8_unit<PLAIN>(unit, g[i], v[i]);
+    f8_store_fours(v, q, left, w);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = at + 128 * j + 4 * lane, n = o.width - c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[4 * j + i] = 0.f;
+    if (n <= 0) continue;
+    if (WAY == 1) {
+      const T* p = row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block);
+      f8_load4(p, n, g + 4 * j);
+      f8_load4(p + block, n, v + 4 * j);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) {
+          const T* p = row + c + i + (size_t)((c + i) / block) * block;
+          g[4 * j + i] = to_float(p[0]), v[4 * j + i] = to_float(p[block]);
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (at + 128 * j + 4 * lane < o.width) {      // (behind the row's end the unit of zeros need not be zero)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * j + i] = at + 128 * j + 4 * lane + i < o.width ? f8_unit<PLAIN>(unit, g[4 * j + i], v[4 * j + i]) : 0.f;
+    }
+  f8_store_fours(v, q, left, w);
 }
 
 // ---- the residual sum and the norm ------------------------------------------------------------------------------------
@@ -176,52 +272,103 @@ __device__ __forceinline__ float f8_inverse_root(double mean) {
   return (float)(y * (1.5 - 0.5 * mean * y * y));
 }
 
-// A thread keeps 16 consecutive numbers of the row in registers (rows of at most 16,384 numbers, 16 at a time).
-template <typename T>
-__global__ void __launch_bounds__(1024)
-f8_norm_runs_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight,
-                    const int* __restrict__ rows, int h_rows, float eps, double per, const F8Rows o) {
+// Rows of at most 16,384 numbers: a warp keeps the 512 numbers of its word in registers between the sum and the result.
+template <typename T, bool RUNS, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 512 ? 3 : 1)
+f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight, const int* __restrict__ rows,
+               int h_rows, float eps, double per, const F8Rows o) {
   __shared__ double red[32];
   pdl_launch_dependents();
   pdl_wait();
-  const int r = blockIdx.x, c = threadIdx.x * 16, from = rows ? rows[r] : r;
-  const bool live = c < o.width && from >= 0 && from < h_rows;
+  const int r = blockIdx.x, lane = threadIdx.x & 31, word = threadIdx.x >> 5, from = rows ? rows[r] : r;
+  const bool live = from >= 0 && from < h_rows;
+  const int at = word * F8_WORD, left = live ? o.width - at : 0;
+  float* hr = h + (live ? (size_t)from * o.width + at : 0);
+  const T* dr = delta ? delta + (live ? (size_t)from * o.width + at : 0) : nullptr;
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  float ss = 0.f;
-  if (live) {
-    float* hr = h + (size_t)from * o.width + c;
-    f8_load16(hr, v);
-    if (delta) {
-      float d[16];
-      f8_load16(delta + (size_t)from * o.width + c, d);
+  if (RUNS) {
+    if (16 * lane < left) {
+      f8_load16(hr + 16 * lane, v);
+      if (dr) {
+        float d[16];
+        f8_load16(dr + 16 * lane, d);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] += d[i];
-      if (!rows) {
+        for (int i = 0; i < 16; ++i) v[i] += d[i];
+        if (!rows) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(hr + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(hr + 16 * lane + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
       }
     }
+  } else {
+    float d[16];
+    if (left >= F8_WORD) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-  }
-  const double total = f8_block_sum((double)ss, red);
-  const float inv = f8_inverse_root(total * per + (double)eps);
-  if (live) {
-    float wt[16];
-    f8_load16(weight + c, wt);
+      for (int j = 0; j < 4; ++j) f8_load4(hr + 128 * j + 4 * lane, 4, v + 4 * j);
+      if (dr) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = v[i] * inv * wt[i];
+        for (int j = 0; j < 4; ++j) f8_load4(dr + 128 * j + 4 * lane, 4, d + 4 * j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = 128 * j + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[4 * j + i] = 0.f;
+        if (c < left) f8_load4(hr + c, left - c, v + 4 * j);
+        if (dr && c < left) f8_load4(dr + c, left - c, d + 4 * j);
+      }
+    }
+    if (dr) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = 128 * (i / 4) + 4 * lane + i % 4;
+        v[i] += d[i];
+        if (!rows && c < left) hr[c] = v[i];
+      }
+    }
   }
-  const int word = threadIdx.x >> 5;
-  f8_store_runs(v, c < o.width ? o.q + (size_t)r * o.pitch + c : nullptr, o.words + (size_t)word * o.rows + r);
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
+  const float inv = f8_inverse_root(f8_block_sum((double)ss, red) * per + (double)eps);
+  float wt[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) wt[i] = 0.f;
+  if (RUNS) {
+    if (16 * lane < left) f8_load16(weight + at + 16 * lane, wt);
+  } else {
+    if (left >= F8_WORD) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f8_load4(weight + at + 128 * j + 4 * lane, 4, wt + 4 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (128 * j + 4 * lane < left) f8_load4(weight + at + 128 * j + 4 * lane, left - 128 * j - 4 * lane, wt + 4 * j);
+    }
+  }
+  const int there = o.width - at;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int c = RUNS ? 16 * lane : 128 * (i / 4) + 4 * lane + i % 4;
+    v[i] = c < left ? v[i] * inv * wt[i] : 0.f;      // (inv may be no number)
+  }
+  uint8_t* q = o.q + (size_t)r * o.pitch + at;
+  uint32_t* w = o.words + (size_t)word * o.rows + r;
+  if (RUNS)
+    f8_store_runs(v, 16 * lane < there ? q + 16 * lane : nullptr, w);
+  else
+    f8_store_fours(v, q, there, w);
 }
 
+// Longer rows: read again between the two.
 constexpr int F8_NORM_THREADS = 512;
 template <typename T>
 __global__ void __launch_bounds__(F8_NORM_THREADS)
-f8_norm_dealt_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight,
+f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight,
                      const int* __restrict__ rows, int h_rows, float eps, double per, const F8Rows o) {
   __shared__ double red[32];
   pdl_launch_dependents();
@@ -247,7 +394,7 @@ f8_norm_dealt_kernel(float* __restrict__ h, const T* __restrict__ delta, const f
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int c = at + lane + 32 * i;
+      const int c = at + 128 * (i / 4) + 4 * lane + i % 4;
       v[i] = 0.f;
       if (live && c < o.width) {
         v[i] = hr[c];
@@ -255,7 +402,7 @@ f8_norm_dealt_kernel(float* __restrict__ h, const T* __restrict__ delta, const f
         v[i] = v[i] * inv * weight[c];
       }
     }
-    f8_store_dealt(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);
+    f8_store_fours(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);
   }
 }
 
@@ -271,7 +418,10 @@ static int f8_rows_of(F8Rows* o, const char* what, void* q, long long pitch, voi
 static bool f8_in_runs(const void* x, long long stride, int size, int width) {
   return width % 16 == 0 && ((uintptr_t)x & 31) == 0 && stride * size % 32 == 0;
 }
-static dim3 f8_grid(const F8Rows& o) { return dim3((unsigned)((o.rows - 1) / (F8_THREADS / 32) + 1), (unsigned)o.n_words); }
+// Blocks of eight rows and `words` words.
+static dim3 f8_grid(const F8Rows& o, int words) {
+  return dim3((unsigned)((o.rows - 1) / (F8_THREADS / 32) + 1), (unsigned)((o.n_words - 1) / words + 1));
+}
 
 LLMRS_API int llmrs_quantize_fp8(const void* x, int dtype, long long x_stride, int x_rows, const int* src, void* q,
                                  long long pitch, void* words, int rows, int width, cudaStream_t stream) {
@@ -281,15 +431,27 @@ LLMRS_API int llmrs_quantize_fp8(const void* x, int dtype, long long x_stride, i
   cudaError_t e;
   if (dtype == LLMRS_F32) {
     auto* k = f8_in_runs(x, x_stride, 4, width) ? f8_quantize_kernel<float, true> : f8_quantize_kernel<float, false>;
-    e = llmrs_launch(k, f8_grid(o), dim3(F8_THREADS), 0, stream, true, (const float*)x, x_stride, x_rows, src, o);
+    e = llmrs_launch(k, f8_grid(o, 2), dim3(F8_THREADS), 0, stream, true, (const float*)x, x_stride, x_rows, src, o);
   } else if (dtype == LLMRS_BF16) {
     auto* k = f8_in_runs(x, x_stride, 2, width) ? f8_quantize_kernel<__nv_bfloat16, true> : f8_quantize_kernel<__nv_bfloat16, false>;
-    e = llmrs_launch(k, f8_grid(o), dim3(F8_THREADS), 0, stream, true, (const __nv_bfloat16*)x, x_stride, x_rows, src, o);
+    e = llmrs_launch(k, f8_grid(o, 2), dim3(F8_THREADS), 0, stream, true, (const __nv_bfloat16*)x, x_stride, x_rows, src, o);
   } else {
     return llmrs_fail("quantize_fp8: unknown dtype %d", dtype);
   }
   if (e != cudaSuccess) return llmrs_fail("quantize_fp8 launch: %s", cudaGetErrorString(e));
   return llmrs_launch_status("quantize_fp8");
+}
+
+template <typename T>
+static cudaError_t f8_launch_unit(const T* gu, long long gu_stride, int block, const GatedUnit& unit, const F8Rows& o,
+                                  cudaStream_t stream) {
+  const bool plain = unit.limit == INFINITY && unit.alpha == 1.0f && unit.shift == 0.0f;
+  const int shift = block & (block - 1) ? -1 : __builtin_ctz((unsigned)block);
+  const int way = block % 16 == 0 && f8_in_runs(gu, gu_stride, (int)sizeof(T), o.width) ? 0 : block == o.width || block % 4 == 0 ? 1 : 2;
+  auto* k = way == 0   ? (plain ? f8_unit_kernel<T, 0, true> : f8_unit_kernel<T, 0, false>)
+            : way == 1 ? (plain ? f8_unit_kernel<T, 1, true> : f8_unit_kernel<T, 1, false>)
+                       : (plain ? f8_unit_kernel<T, 2, true> : f8_unit_kernel<T, 2, false>);
+  return llmrs_launch(k, f8_grid(o, 1), dim3(F8_THREADS), 0, stream, true, gu, gu_stride, block, shift, unit, o);
 }
 
 // gu [rows, 2 * width]: gate and up in alternating runs of `block` columns (which divides the width).
@@ -300,17 +462,13 @@ LLMRS_API int llmrs_silu_mul_fp8(const void* gu, int dtype, long long gu_stride,
   LLMRS_REQUIRE(block > 0 && width % block == 0, "silu_mul_fp8: runs of %d columns do not divide %d", block, width);
   if (rows == 0) return 0;
   const GatedUnit unit = {limit, alpha, shift};
-  const bool runs = block % 16 == 0;
   cudaError_t e;
-  if (dtype == LLMRS_F32) {
-    auto* k = runs && f8_in_runs(gu, gu_stride, 4, width) ? f8_unit_kernel<float, true> : f8_unit_kernel<float, false>;
-    e = llmrs_launch(k, f8_grid(o), dim3(F8_THREADS), 0, stream, true, (const float*)gu, gu_stride, block, unit, o);
-  } else if (dtype == LLMRS_BF16) {
-    auto* k = runs && f8_in_runs(gu, gu_stride, 2, width) ? f8_unit_kernel<__nv_bfloat16, true> : f8_unit_kernel<__nv_bfloat16, false>;
-    e = llmrs_launch(k, f8_grid(o), dim3(F8_THREADS), 0, stream, true, (const __nv_bfloat16*)gu, gu_stride, block, unit, o);
-  } else {
+  if (dtype == LLMRS_F32)
+    e = f8_launch_unit((const float*)gu, gu_stride, block, unit, o, stream);
+  else if (dtype == LLMRS_BF16)
+    e = f8_launch_unit((const __nv_bfloat16*)gu, gu_stride, block, unit, o, stream);
+  else
     return llmrs_fail("silu_mul_fp8: unknown dtype %d", dtype);
-  }
   if (e != cudaSuccess) return llmrs_fail("silu_mul_fp8 launch: %s", cudaGetErrorString(e));
   return llmrs_launch_status("silu_mul_fp8");
 }
@@ -318,13 +476,16 @@ LLMRS_API int llmrs_silu_mul_fp8(const void* gu, int dtype, long long gu_stride,
 template <typename T>
 static cudaError_t f8_launch_norm(float* h, const T* delta, const float* weight, const int* rows, int h_rows, float eps,
                                   const F8Rows& o, cudaStream_t stream) {
-  const bool runs = o.width <= 16384 && f8_in_runs(h, o.width, 4, o.width) && ((uintptr_t)weight & 31) == 0 &&
+  const double per = 1.0 / o.width;
+  if (o.n_words > 32)
+    return llmrs_launch(f8_norm_long_kernel<T>, dim3(o.rows), dim3(F8_NORM_THREADS), 0, stream, true, h, delta, weight, rows, h_rows,
+                        eps, per, o);
+  const bool runs = f8_in_runs(h, o.width, 4, o.width) && ((uintptr_t)weight & 31) == 0 &&
                     (!delta || f8_in_runs(delta, o.width, (int)sizeof(T), o.width));
-  if (runs)
-    return llmrs_launch(f8_norm_runs_kernel<T>, dim3(o.rows), dim3(o.n_words * 32), 0, stream, true, h, delta, weight, rows, h_rows,
-                        eps, 1.0 / o.width, o);
-  return llmrs_launch(f8_norm_dealt_kernel<T>, dim3(o.rows), dim3(F8_NORM_THREADS), 0, stream, true, h, delta, weight, rows, h_rows,
-                      eps, 1.0 / o.width, o);
+  auto* k = o.n_words <= 16 ? (runs ? f8_norm_kernel<T, true, 512> : f8_norm_kernel<T, false, 512>)
+                            : (runs ? f8_norm_kernel<T, true, 1024> : f8_norm_kernel<T, false, 1024>);
+  return llmrs_launch(k, dim3(o.rows), dim3(o.n_words * 32), 0, stream, true,
+                      h, delta, weight, rows, h_rows, eps, per, o);
 }
 
 // h [h_rows, width] float32 and delta (or null) of `dtype`, contiguous.
