@@ -1973,21 +1973,23 @@ def _fp8_stream(*tensors) -> int:
     return _raw_stream(current) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-def _fp8_rows(x: torch.Tensor, name: str) -> int:
-    """The row stride of a matrix of float32 or bfloat16 with dense rows."""
-    if x.dtype not in _DTYPE_CODE:
+def _fp8_rows(x: torch.Tensor, name: str):
+    """(rows, columns, row stride, type) of a matrix of float32 or bfloat16 with dense rows."""
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None:
         raise KernelError(f"{name}: kernels take float32 or bfloat16, not {x.dtype}")
     if x.dim() != 2 or x.size(1) < 1:
         raise KernelError(f"{name} must be [rows, numbers], got {tuple(x.shape)}")
+    rows, K = x.shape
     stride, one = x.stride()
-    if one != 1 and x.size(1) > 1:
+    if one != 1 and K > 1:
         raise KernelError(f"{name} must have dense rows, got sizes {tuple(x.shape)} strides {x.stride()}")
-    return x.size(1) if x.size(0) == 1 else stride
+    return rows, K, K if rows == 1 else stride, code
 
 
 def _fp8_operand(q: torch.Tensor, scales: torch.Tensor, name: str):
-    """(bytes between rows, words between the scales of neighbouring words) of rows in 8 bits."""
-    if q.dtype != FP8 or scales.dtype != FP8_SCALE:
+    """(rows, K, address, bytes between rows, scales' address, words between the scales of neighbouring words) of rows in 8 bits."""
+    if q.dtype is not FP8 or scales.dtype is not FP8_SCALE:
         raise KernelError(f"{name} must be {FP8} with scales of {FP8_SCALE}, got {q.dtype} with {scales.dtype}")
     if q.dim() != 2 or q.size(1) < 1:
         raise KernelError(f"{name} must be [rows, K], got {tuple(q.shape)}")
@@ -1995,28 +1997,28 @@ def _fp8_operand(q: torch.Tensor, scales: torch.Tensor, name: str):
     words = (K + 511) >> 9
     if scales.shape != (words, rows, 4):
         raise KernelError(f"{name} is {tuple(q.shape)}: its scales must be {(words, rows, 4)}, got {tuple(scales.shape)}")
-    if rows == 0:
-        return (K + 15) & -16, 0
     pitch, one = q.stride()
-    if rows == 1:
-        pitch = (K + 15) & -16
-    if (K > 1 and one != 1) or pitch % 16 or pitch < K or q.data_ptr() % 16:
-        raise KernelError(f"{name}: rows must be dense and start at multiples of 16 bytes, got strides {q.stride()}")
     stride, row, byte = scales.stride()
+    if rows <= 1:       # strides of one row, of one column, of one word say nothing
+        pitch, row = (K + 15) & -16, 4
+    if K == 1:
+        one = 1
     if words == 1:
         stride = 4 * rows
-    if byte != 1 or (rows > 1 and row != 4) or stride % 4 or stride < 0 or scales.data_ptr() % 4:
+    at, scales_at = q.data_ptr(), scales.data_ptr()
+    if rows and (one != 1 or (pitch | at) & 15 or pitch < K):
+        raise KernelError(f"{name}: rows must be dense and start at multiples of 16 bytes, got strides {q.stride()}")
+    if rows and (byte != 1 or row != 4 or (stride | scales_at) & 3 or stride < 0):
         raise KernelError(f"{name}: a word of four scales must be dense, and words of neighbouring rows adjacent, got strides "
                           f"{scales.stride()}")
-    return pitch, stride >> 2
+    return rows, K, at, pitch, scales_at, stride >> 2
 
 
 def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
     """Rows of float32 or bfloat16 ``x`` [rows, K] (dense rows, any stride) in 8 bits: ``(q, scales)`` as above, each number
     rounded once, to nearest. A NaN or an infinity becomes a NaN. ``src`` (int32): row i is made from row ``src[i]`` of x (one row
     may be named often; an index that names none of x's rows gives zeros). Weights are quantised by the same call."""
-    stride = _fp8_rows(x, "x")
-    rows, K = x.shape
+    rows, K, stride, code = _fp8_rows(x, "x")
     if src is not None:
         if src.dtype != torch.int32 or src.dim() != 1 or not src.is_contiguous():
             raise KernelError(f"src must be a contiguous int32 vector, got {src.dtype} {tuple(src.shape)}")
@@ -2024,7 +2026,7 @@ def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
     n = rows if src is None else src.numel()
     q, scales, pitch = _fp8_new(x, n, K)
     fn = _fp8_entries.get("llmrs_quantize_fp8") or _fp8_entry("llmrs_quantize_fp8", 11, wide=(0, 2, 4, 5, 6, 7, 10))
-    _check(fn(x.data_ptr(), _DTYPE_CODE[x.dtype], stride, rows, None if src is None else src.data_ptr(), q.data_ptr(), pitch,
+    _check(fn(x.data_ptr(), code, stride, rows, None if src is None else src.data_ptr(), q.data_ptr(), pitch,
               scales.data_ptr(), n, K, stream), "quantize_fp8")
     return q, scales
 
@@ -2033,15 +2035,14 @@ def silu_mul_fp8(gate_up: torch.Tensor, block: int = 0, unit=PLAIN_SILU):
     """``silu_mul`` with its result in 8 bits: ``(q, scales)`` of ``silu(gate) * up`` for ``gate_up`` [rows, 2I] that holds gate and
     up in alternating runs of ``block`` columns (0: I gate columns, then I up columns; else a divisor of I). The unit is
     computed in float32 and rounded once."""
-    stride_in = _fp8_rows(gate_up, "gate_up")
-    rows, two = gate_up.shape
+    rows, two, stride, code = _fp8_rows(gate_up, "gate_up")
     inter = two // 2
     if two % 2 or block < 0 or (block and inter % block):
         raise KernelError(f"gate_up has {two} columns: not two times a multiple of runs of {block}")
     stream = _fp8_stream(gate_up)
     q, scales, pitch = _fp8_new(gate_up, rows, inter)
     fn = _fp8_entries.get("llmrs_silu_mul_fp8") or _fp8_entry("llmrs_silu_mul_fp8", 13, (4, 5, 6), (0, 2, 7, 8, 9, 12))
-    _check(fn(gate_up.data_ptr(), _DTYPE_CODE[gate_up.dtype], stride_in, block or inter, *unit, q.data_ptr(), pitch,
+    _check(fn(gate_up.data_ptr(), code, stride, block or inter, *unit, q.data_ptr(), pitch,
               scales.data_ptr(), rows, inter, stream), "silu_mul_fp8")
     return q, scales
 
@@ -2054,8 +2055,7 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
     for name, t in (("h", h), ("weight", weight)):
         if t.dtype != torch.float32 or not t.is_contiguous():
             raise KernelError(f"{name} must be contiguous float32, got {t.dtype}")
-    _fp8_rows(h, "h")
-    n, K = h.shape
+    n, K, _, _ = _fp8_rows(h, "h")
     if weight.numel() != K:
         raise KernelError(f"norm weight has {weight.numel()} elements, rows have {K}")
     if delta is not None and (delta.dtype not in _DTYPE_CODE or delta.shape != h.shape or not delta.is_contiguous()):
@@ -2073,8 +2073,7 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
 
 
 def _fp8_product():
-    return _fp8_entries.get("llmrs_gemm_fp8") or _fp8_entry("llmrs_gemm_fp8", 24,
-                                                            wide=(0, 1, 2, 3, 5, 6, 7, 8, 9, 10, 16, 17, 22, 23))
+    return _fp8_entry("llmrs_gemm_fp8", 24, wide=(0, 1, 2, 3, 5, 6, 7, 8, 9, 10, 16, 17, 22, 23))
 
 
 def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
@@ -2082,33 +2081,30 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     """``x @ w.T`` of rows in 8 bits, ``x`` [tokens, K] and ``w`` [features, K] (``quantize_fp8``), on tcgen05 with the scales applied
     by the tensor core and float32 sums (see csrc/gemm_fp8.cu). Epilogue "store": [tokens, features] in ``out_dtype`` (bfloat16 or
     float32), into ``out`` when given. "residual": ``out``, the float32 residual stream, gets the product added."""
-    x_pitch, xs = _fp8_operand(x, x_scales, "x")
-    w_pitch, ws = _fp8_operand(w, w_scales, "w")
-    tokens, K = x.shape
-    features = w.size(0)
-    if w.size(1) != K:
-        raise KernelError(f"x has {K} columns, w has {w.size(1)}")
+    tokens, K, x_at, x_pitch, xs_at, xs = _fp8_operand(x, x_scales, "x")
+    features, w_K, w_at, w_pitch, ws_at, ws = _fp8_operand(w, w_scales, "w")
+    if w_K != K:
+        raise KernelError(f"x has {K} columns, w has {w_K}")
     if features < 1:
         raise KernelError("w has no rows")
-    if epilogue not in ("store", "residual"):
-        raise KernelError(f"unknown epilogue {epilogue!r}: 'store' or 'residual'")
     add = epilogue == "residual"
-    if add and out is None:
-        raise KernelError("the residual epilogue needs the stream it adds to as out")
+    if not add and epilogue != "store":
+        raise KernelError(f"unknown epilogue {epilogue!r}: 'store' or 'residual'")
     if out is None:
-        dtype_code(out_dtype)
+        if add:
+            raise KernelError("the residual epilogue needs the stream it adds to as out")
+        code = dtype_code(out_dtype)
         stream = _fp8_stream(x, x_scales, w, w_scales)
-        out = x.new_empty((tokens, features), dtype=out_dtype)
+        out, ldo = x.new_empty((tokens, features), dtype=out_dtype), features
     else:
         if out.dtype != (torch.float32 if add else out_dtype) or out.shape != (tokens, features):
             raise KernelError(f"out is {tuple(out.shape)} {out.dtype}, the product {(tokens, features)} "
                               f"{torch.float32 if add else out_dtype}")
-        dtype_code(out.dtype)
-        _row_stride(out, "out")
+        code, ldo = dtype_code(out.dtype), _row_stride(out, "out")
         stream = _fp8_stream(x, x_scales, w, w_scales, out)
-    _check(_fp8_product()(x.data_ptr(), x_pitch, x_scales.data_ptr(), xs, tokens, w.data_ptr(), w_pitch, w_scales.data_ptr(), ws,
-                          out.data_ptr(), out.stride(0), _DTYPE_CODE[out.dtype], add, features, K, 1, None, None, 0, 0, 0, 0,
-                          tc_error_flag(x.device).data_ptr(), stream), "gemm_fp8")
+    _check((_fp8_entries.get("llmrs_gemm_fp8") or _fp8_product())(
+        x_at, x_pitch, xs_at, xs, tokens, w_at, w_pitch, ws_at, ws, out.data_ptr(), ldo, code, add, features, K, 1, None, None, 0, 0,
+        0, 0, tc_error_flag(x.device).data_ptr(), stream), "gemm_fp8")
     return out
 
 
@@ -2127,16 +2123,15 @@ def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     device; both from ``moe_sort``). ``w`` is [groups, features, K], ``w_scales`` [ceil(K / 512), groups * features, 4]: what
     ``quantize_fp8`` makes of the groups' rows under one another. ``out`` [rows, features] is bfloat16 or float32; rows that no
     tile names are left as they are. A tile that names a group or a first row that is not there computes nothing."""
-    x_pitch, xs = _fp8_operand(x, x_scales, "x")
+    rows, x_K, x_at, x_pitch, xs_at, xs = _fp8_operand(x, x_scales, "x")
     if w.dim() != 3 or w.size(0) < 1 or w.size(1) < 1:
         raise KernelError(f"w must be [groups, features, K], got {tuple(w.shape)}")
     G, N, K = w.shape
     if G > 1 and N > 1 and w.stride(0) != N * w.stride(1):
         raise KernelError(f"w: the groups' rows must lie under one another, got strides {w.stride()}")
-    w_pitch, ws = _fp8_operand(w.flatten(0, 1), w_scales, "w")
-    rows = x.size(0)
-    if x.size(1) != K:
-        raise KernelError(f"x has {x.size(1)} columns, w has {K}")
+    _, _, w_at, w_pitch, ws_at, ws = _fp8_operand(w.flatten(0, 1), w_scales, "w")
+    if x_K != K:
+        raise KernelError(f"x has {x_K} columns, w has {K}")
     if out.shape != (rows, N) or out.dtype not in _DTYPE_CODE:
         raise KernelError(f"out is {tuple(out.shape)} {out.dtype}, the product {(rows, N)} in float32 or bfloat16")
     _row_stride(out, "out")
@@ -2147,7 +2142,8 @@ def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     if n_tiles.dtype != torch.int32 or n_tiles.numel() != 1:
         raise KernelError(f"n_tiles must be one int32, got {n_tiles.dtype} {tuple(n_tiles.shape)}")
     stream = _fp8_stream(x, x_scales, w, w_scales, out, tiles, n_tiles)
-    _check(_fp8_product()(x.data_ptr(), x_pitch, x_scales.data_ptr(), xs, rows, w.data_ptr(), w_pitch, w_scales.data_ptr(), ws,
-                          out.data_ptr(), out.stride(0), _DTYPE_CODE[out.dtype], 0, N, K, G, tiles.data_ptr(), n_tiles.data_ptr(),
-                          tiles.size(0), tile_rows, 0, 0, tc_error_flag(x.device).data_ptr(), stream), "gemm_fp8_grouped")
+    _check((_fp8_entries.get("llmrs_gemm_fp8") or _fp8_product())(
+        x_at, x_pitch, xs_at, xs, rows, w_at, w_pitch, ws_at, ws, out.data_ptr(), out.stride(0), _DTYPE_CODE[out.dtype], 0, N, K, G,
+        tiles.data_ptr(), n_tiles.data_ptr(), tiles.size(0), tile_rows, 0, 0, tc_error_flag(x.device).data_ptr(), stream),
+        "gemm_fp8_grouped")
     return out
