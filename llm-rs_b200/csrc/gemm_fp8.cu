@@ -309,20 +309,28 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_slot)), "r"(C::COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (tid == 64 && !p.tiles) {
     // The first weights on their way into the L2 while the kernel before this one ends (a hint: they are copied only after it).
     for (int kb = kb0; kb < kb1 && kb < kb0 + 2 * p.stages; ++kb) g8_prefetch(&map_w, kb * G8_BK, (int)blockIdx.x / p.n_t * G8_BM);
   }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
   if (splits > 1) g8_cluster_arrive();
-  const uint32_t tmem_base = *tmem_slot, tmem_scales = tmem_base + C::ACC_COLS;
   pdl_wait();      // everything below reads or writes what earlier kernels may have touched
+  // Tensor memory is asked for after the wait: a block that held some while it waits for an earlier kernel could keep that kernel's
+  // blocks from theirs. The copies start meanwhile.
+  uint32_t tmem_base = 0;
+  if (warp >= 1) {
+    if (warp == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_slot)), "r"(C::COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 2, %0;" ::"n"(G8F_THREADS - 32) : "memory");
+    tc_fence_after();
+    tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  }
+  const uint32_t tmem_scales = tmem_base + C::ACC_COLS;
   const int n_row_tiles = p.tiles ? min(*p.n_tiles, p.max_tiles) : p.n_t;
   const bool live = blockIdx.x < (long long)n_row_tiles * p.n_f;      // (a list's tiles may be fewer than the grid has room for)
   const G8Tile w = live ? g8_tile(p, blockIdx.x, n_row_tiles, G8_BM) : G8Tile{0, 0, 0, 0};
@@ -612,17 +620,22 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_slot)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
   __syncthreads();
   g8_cluster_arrive();      // the peer's barriers exist before anything is sent to them
   g8_cluster_wait();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot, tmem_scales = tmem_base + G8P_NT;
   pdl_wait();
+  uint32_t tmem_base = 0;      // (asked for after the wait, see above; the same columns in both blocks)
+  if (warp >= 1) {
+    if (warp == 1) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_slot)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 2, %0;" ::"n"(G8P_THREADS - 32) : "memory");
+    tc_fence_after();
+    tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  }
+  const uint32_t tmem_scales = tmem_base + G8P_NT;
   const int n_row_tiles = p.tiles ? min(*p.n_tiles, p.max_tiles) : p.n_t, n_work = n_row_tiles * p.n_f;
   int copies = 0;      // stages whose copies this block has requested
 
