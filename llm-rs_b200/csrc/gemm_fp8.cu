@@ -66,6 +66,17 @@ __device__ __forceinline__ void g8_st4(uint32_t taddr, const uint32_t (&v)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
 }
+// 16 consecutive float32 columns of this thread's lane.
+__device__ __forceinline__ void g8_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void g8_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -526,13 +537,15 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 // issues the MMAs of both.
 //   full[s], scales_full[s]    (leader's) both blocks' copies, or words, of a stage or slot are there
 //   empty[s], scales_empty[s]  (each block's) the MMAs that read it are done
-//   acc_full                   (each block's) the tile's sums are complete;  acc_empty (leader's): both epilogues have read them
-// Warps 2-5 write the words of scales, warps 6-13 run the epilogue: a quarter of the rows and half of the columns each. The
-// accumulator is one of 256 columns (with the words of scales there is no room for two): an epilogue warp keeps its bfloat16
-// results in registers and gives tensor memory back before it stores.
+//   acc_full[2]                (each block's) the tile's sums are complete;  acc_empty[2] (leader's): both epilogues have read them
+// Warps 2-5 write the words of scales, warps 6-13 run the epilogue: a quarter of the rows and half of the columns each. The words of
+// scales leave 464 columns of tensor memory for the sums: every other tile has its at the lower end, the others at the upper, so
+// that a tile's epilogue runs under the next one's MMAs wherever two neighbours have 464 tokens or fewer; else the next tile
+// waits until this one's sums are read (an epilogue warp keeps its bfloat16 results in registers and gives tensor memory back
+// before it stores).
 constexpr int G8P_THREADS = 448, G8P_EPI_WARP = 6, G8P_STAGES = 6, G8P_NT = 256;
 constexpr uint32_t G8P_STAGE_BYTES = G8_A_BYTES + G8P_NT / 2 * G8_BK;
-constexpr int G8P_SLOT_COLS = 12, G8P_BARS = 2 * G8P_STAGES + 2 * G8_SLOTS + 3;
+constexpr int G8P_SLOT_COLS = 12, G8P_SUM_COLS = 512 - G8_SLOTS * G8P_SLOT_COLS, G8P_BARS = 2 * G8P_STAGES + 2 * G8_SLOTS + 5;
 constexpr size_t G8P_SMEM = 1024 + (size_t)G8P_STAGES * G8P_STAGE_BYTES + G8P_BARS * 8 + 16;
 
 // A copy into this block's shared memory whose bytes are counted by a barrier that may lie in the pair's other block.
@@ -601,8 +614,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t full0 = tc_smem(bars), empty0 = full0 + 8 * G8P_STAGES, sc_full0 = empty0 + 8 * G8P_STAGES,
-                 sc_empty0 = sc_full0 + 8 * G8_SLOTS, acc_full = sc_empty0 + 8 * G8_SLOTS, acc_empty = acc_full + 8,
-                 drain_bar = acc_empty + 8;
+                 sc_empty0 = sc_full0 + 8 * G8_SLOTS, acc_full = sc_empty0 + 8 * G8_SLOTS, acc_empty = acc_full + 16,
+                 drain_bar = acc_empty + 16;
   const uint32_t rank = g8_rank();      // 0: the leader
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, nkb = p.nkb;
 
@@ -610,7 +623,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   if (warp == 0) {
     for (int s = lane; s < G8P_BARS; s += 32) {      // four, or eight, warps of both blocks arrive on two of the kinds
       const uint32_t bar = full0 + 8 * s;
-      mbar_init(bar, bar >= sc_full0 && bar < sc_empty0 ? 8 : bar == acc_empty ? 16 : 1);
+      mbar_init(bar, bar >= sc_full0 && bar < sc_empty0 ? 8 : bar >= acc_empty && bar < drain_bar ? 16 : 1);
     }
     if (lane == 0) {
       g8_prefetch_map(&map_w);
@@ -635,7 +648,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     tc_fence_after();
     tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   }
-  const uint32_t tmem_scales = tmem_base + G8P_NT;
+  const uint32_t tmem_scales = tmem_base + G8P_SUM_COLS;
   const int n_row_tiles = p.tiles ? min(*p.n_tiles, p.max_tiles) : p.n_t, n_work = n_row_tiles * p.n_f;
   int copies = 0;      // stages whose copies this block has requested
 
@@ -667,12 +680,17 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (rank == 0 && tc_elect_one()) {
       G8Ring r(G8P_STAGES);
       G8Ring sc(G8_SLOTS);
-      uint32_t acc_phase = 1;
       bool ok = true;
-      for (int t = pair; t < n_work && ok; t += n_pairs, acc_phase ^= 1) {
-        const uint32_t idesc0 = g8_idesc(2 * G8_BM, g8_pair_n(g8_tile(p, t, n_row_tiles, 2 * G8_BM).rows), 0);
-        ok = g8_wait_cluster(acc_empty, acc_phase, p.wait_limit, abort_flag);      // both epilogues have read the tile before
+      int lt = 0, before = 0;      // tiles so far, tokens of the last one's MMAs
+      for (int t = pair; t < n_work && ok; t += n_pairs, ++lt) {
+        const int n = g8_pair_n(g8_tile(p, t, n_row_tiles, 2 * G8_BM).rows), end = lt & 1;
+        const uint32_t idesc0 = g8_idesc(2 * G8_BM, n, 0), d_addr = tmem_base + (end ? G8P_SUM_COLS - n : 0);
+        // Both epilogues have read the tile that lay at this end, and the one at the other where this one reaches into it.
+        ok = g8_wait_cluster(acc_empty + 8 * end, (uint32_t)((lt >> 1) & 1) ^ 1, p.wait_limit, abort_flag);
+        if (ok && before + n > G8P_SUM_COLS)
+          ok = g8_wait_cluster(acc_empty + 8 * (1 - end), (uint32_t)((lt - 1) >> 1) & 1, p.wait_limit, abort_flag);
         if (!ok) break;
+        before = n;
         tc_fence_after();
         uint32_t acc = 0;
         for (int kb = 0; kb < nkb && ok; kb += 4, sc.next()) {      // a word of scales
@@ -688,7 +706,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             const uint64_t a_desc = tc_smem_desc(a_addr), b_desc = tc_smem_desc(a_addr + G8_A_BYTES);
 #pragma unroll
             for (int k = 0; k < G8_BK / 32; ++k) {
-              g8_mma_pair(tmem_base, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, sa, sa + 4, acc);
+              g8_mma_pair(d_addr, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, sa, sa + 4, acc);
               acc = 1;
             }
             g8_commit_pair(empty0 + 8 * r.at);
@@ -696,7 +714,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           }
           g8_commit_pair(sc_empty0 + 8 * sc.at);
         }
-        if (ok) g8_commit_pair(acc_full);
+        if (ok) g8_commit_pair(acc_full + 8 * end);
       }
     }
     __syncwarp();
@@ -730,38 +748,39 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
   } else {
     const int quarter = warp & 3, c0 = (warp - G8P_EPI_WARP) / 4 * (G8P_NT / 2);
-    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0;
-    uint32_t phase = 0;
     bool ok = true;
-    for (int t = pair; t < n_work && ok; t += n_pairs, phase ^= 1) {
+    int lt = 0;
+    for (int t = pair; t < n_work && ok; t += n_pairs, ++lt) {
       const G8Tile w = g8_tile(p, t, n_row_tiles, 2 * G8_BM);
       const int n = w.f0 + (int)rank * G8_BM + quarter * 32 + lane, left = min(w.rows - c0, G8P_NT / 2);      // columns of this warp's half
-      ok = __all_sync(0xffffffffu, g8_wait(acc_full, phase, p.wait_limit, abort_flag));
+      const int end = lt & 1;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(c0 + (end ? G8P_SUM_COLS - g8_pair_n(w.rows) : 0));
+      ok = __all_sync(0xffffffffu, g8_wait(acc_full + 8 * end, (uint32_t)(lt >> 1) & 1, p.wait_limit, abort_flag));
       if (!ok) break;
       tc_fence_after();
       if (p.out_f32) {
-        for (int c = 0; c < left; c += 32) {      // all lanes: the reads are warp-wide
-          float v[32];
-          tc_ld32(taddr + c, v);
-          if (n < p.N) g8_store<32>(p, w.m0 + c0 + c, n, left - c, v);
+        for (int c = 0; c < left; c += 16) {      // all lanes: the reads are warp-wide
+          float v[16];
+          g8_ld16(taddr + c, v);
+          if (n < p.N) g8_store<16>(p, w.m0 + c0 + c, n, left - c, v);
           __syncwarp();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) g8_arrive_cluster(g8_map_rank(acc_empty, 0u));
+        if (lane == 0) g8_arrive_cluster(g8_map_rank(acc_empty + 8 * end, 0u));
       } else {
         __nv_bfloat162 keep[G8P_NT / 4];
 #pragma unroll
-        for (int c = 0; c < G8P_NT / 2; c += 32) {
+        for (int c = 0; c < G8P_NT / 2; c += 16) {
           if (c >= left) continue;
-          float v[32];
-          tc_ld32(taddr + c, v);
+          float v[16];
+          g8_ld16(taddr + c, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) keep[c / 2 + e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+          for (int e = 0; e < 8; ++e) keep[c / 2 + e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) g8_arrive_cluster(g8_map_rank(acc_empty, 0u));
+        if (lane == 0) g8_arrive_cluster(g8_map_rank(acc_empty + 8 * end, 0u));
         if (n < p.N) {
           __nv_bfloat16* o = (__nv_bfloat16*)p.out + (size_t)(w.m0 + c0) * p.ldo + n;
 #pragma unroll
@@ -884,14 +903,15 @@ static int g8_launch_few(const CUtensorMap& mw, const CUtensorMap& mx, G8Params&
                    dim3((unsigned)tiles, 1, (unsigned)splits), dim3(1, 1, (unsigned)splits), mw, mx, p, stream);
 }
 
-// The way of a product: tokens a tile (256: on pairs), blocks that share a tile's k, blocks an SM.
-struct G8Choice { int nt, splits, per_sm; };
+// The way of a product: tokens a tile (256: on pairs), blocks that share a tile's k, blocks an SM, tiles of tokens (pairs, dense).
+struct G8Choice { int nt, splits, per_sm, n_t; };
 
 // The microseconds that each way is expected to take, and the way that takes least. What the parts stand for, fitted to products of
 // 1 to 2,048 tokens on a B200 (16 x 128 x 128 takes 2.9 us):
-//   a block copies, and its MMAs take, a block of k in .18 us + .6 ns a token; the blocks of an SM together get some 145 GB/s, all
+//   a block copies, and its MMAs take, a block of k in .18 us + .6 ns a token; the blocks of an SM together get some 138 GB/s, all
 //   together the memory's 6.3 TB/s; a wave of blocks after another starts 2 us late; a split costs .4 us + 35 ns a token of the tile for the exchange of the sums;
-//   a pair of the other kernel takes .35 us + .35 ns a token for a block of k of its 256 features.
+//   a pair of the other kernel takes .25 us + .72 ns a token for a block of k of its 256 features (the copies; the MMAs of 256
+//   tokens are .27), .2 us a tile more, or .8 where two neighbours do not fit tensor memory together.
 // Measured, us (tokens x features x K; NT / splits): 1 x 6,144 x 4,096 16/1 9.4, 16/2 8.1, 16/5 7.7, 16/8 10.7; 32 x 4,096 x 4,096
 // 32/1 8.8, 32/3 7.2, 16/4 7.7; 128 x 6,144 x 4,096 64/1 10.3, 64/2 12.4, 128/1 11.8, pair 17.5; 512 x 4,096 x 4,096 128/1 11.8, 64/1
 // 14.1, pair 17.4; 2,048 x 4,096 x 4,096 pair 31.0, 128/1 37.2.
@@ -899,12 +919,18 @@ struct G8Choice { int nt, splits, per_sm; };
 static G8Choice g8_choose(int rows, int tile_rows, int n_t, int N, int K, long long weight_rows, int sms) {
   const int nkb = (K - 1) / G8_BK + 1;
   const double memory = ((double)weight_rows + rows) * K / 6.3e6;
-  G8Choice best = {256, 1, 1};
-  const long long pair_tiles = (long long)(tile_rows ? n_t : (rows - 1) / 256 + 1) * ((N - 1) / 256 + 1);
-  const int pair_nt = tile_rows ? tile_rows : (int)((rows - 1) / ((rows - 1) / 256 + 1) + 1);
-  const int pairs = sms / 2 > 0 ? sms / 2 : 1;
-  const double pair_walk = (double)((pair_tiles + pairs - 1) / pairs) * nkb * (.35 + .00035 * pair_nt);
-  double least = 5.0 + (pair_walk > memory ? pair_walk : memory);
+  G8Choice best = {256, 1, 1, 0};
+  const int pairs = sms / 2 > 0 ? sms / 2 : 1, pair_f = (N - 1) / 256 + 1;
+  double least = 1e30;
+  const int from = tile_rows ? n_t : (rows - 1) / 256 + 1, to = tile_rows ? n_t : (rows - 1) / 128 + 1;
+  for (int tiles = from; tiles <= to; ++tiles) {      // (more than a few are not tried: the first ones differ most)
+    if (tiles > from + 8) break;
+    const int n = tile_rows ? tile_rows : ((rows - 1) / tiles + 16) & ~15;
+    const double waves = (double)(((long long)tiles * pair_f + pairs - 1) / pairs), step = .25 + .00072 * n;
+    const double walk = waves * (nkb * step + (2 * n > G8P_SUM_COLS ? .8 : .2));
+    const double t = 5.0 + (walk > memory ? walk : memory);
+    if (t < least) least = t, best.n_t = tiles;
+  }
   for (int nt = 16; nt <= 128; nt *= 2) {
     if (tile_rows ? nt < tile_rows : nt >= 2 * rows && nt > 16) continue;
     const long long tiles = (long long)(tile_rows ? n_t : (rows - 1) / nt + 1) * ((N - 1) / G8_BM + 1);
@@ -920,10 +946,10 @@ static G8Choice g8_choose(int rows, int tile_rows, int n_t, int N, int K, long l
         const long long blocks = tiles * splits;
         const double waves = (double)(long long)((blocks + held - 1) / held);
         const int together = per_sm == 2 && blocks > sms ? 2 : 1;
-        const double shared = together * (16.4 + .128 * nt) / 145, alone = .18 + .0006 * nt;
+        const double shared = together * (16.4 + .128 * nt) / 138, alone = .18 + .0006 * nt;
         const double walk = waves * ((nkb + splits - 1) / splits) * (shared > alone ? shared : alone);
         const double t = 3.2 + .004 * nt + (splits > 1 ? .4 + .035 * nt : 0.0) + 2.0 * (waves - 1) + (walk > memory ? walk : memory);
-        if (t < least) least = t, best = {nt, splits, per_sm};
+        if (t < least) least = t, best = {nt, splits, per_sm, 0};
       }
   }
   return best;
@@ -960,10 +986,10 @@ LLMRS_API int llmrs_gemm_fp8(const void* x, long long x_pitch, const void* xs, l
                 what, tile_rows);
   int sms;
   const int dev = g8_device(&sms), nkb = (K - 1) / G8_BK + 1;
-  int per_sm = 0;
+  int per_sm = 0, n_t = 0;
   if (nt == 0) {
     const G8Choice way = g8_chosen(x_rows, tile_rows, max_tiles < x_rows ? max_tiles : x_rows, N, K, (long long)groups * N, sms);
-    nt = way.nt, splits = way.splits, per_sm = way.per_sm;
+    nt = way.nt, splits = way.splits, per_sm = way.per_sm, n_t = way.n_t;
   } else if (splits == 0) {
     splits = 1;
   }
@@ -972,7 +998,7 @@ LLMRS_API int llmrs_gemm_fp8(const void* x, long long x_pitch, const void* xs, l
   G8Params p = {};
   p.out = out, p.ldo = ldo, p.out_f32 = out_dtype == LLMRS_F32, p.epilogue = epilogue;
   p.xs = (const uint32_t*)xs, p.ws = (const uint32_t*)ws, p.xs_stride = xs_stride, p.ws_stride = ws_stride, p.x_rows = x_rows;
-  p.w_rows = groups * N, p.N = N, p.n_f = (N - 1) / (pair ? 2 * G8_BM : G8_BM) + 1, p.n_t = (x_rows - 1) / nt + 1, p.nkb = nkb;
+  p.w_rows = groups * N, p.N = N, p.n_f = (N - 1) / (pair ? 2 * G8_BM : G8_BM) + 1, p.n_t = n_t > 0 && pair && !grouped ? n_t : (x_rows - 1) / nt + 1, p.nkb = nkb;
   // Dense: tiles of one size, and one copy of their rows a stage; a list's tiles are ragged, their rows come 32 at a time.
   p.nt = grouped ? nt : ((x_rows - 1) / p.n_t + 16) & ~15;
   p.x_box = grouped ? (nt < 32 ? nt : 32) : (pair ? p.nt / 2 : p.nt);
