@@ -998,9 +998,11 @@ LLMRS_API int llmrs_gemm_fp8(const void* x, long long x_pitch, const void* xs, l
   G8Params p = {};
   p.out = out, p.ldo = ldo, p.out_f32 = out_dtype == LLMRS_F32, p.epilogue = epilogue;
   p.xs = (const uint32_t*)xs, p.ws = (const uint32_t*)ws, p.xs_stride = xs_stride, p.ws_stride = ws_stride, p.x_rows = x_rows;
-  p.w_rows = groups * N, p.N = N, p.n_f = (N - 1) / (pair ? 2 * G8_BM : G8_BM) + 1, p.n_t = n_t > 0 && pair && !grouped ? n_t : (x_rows - 1) / nt + 1, p.nkb = nkb;
+  p.w_rows = groups * N, p.N = N, p.nkb = nkb, p.n_f = (N - 1) / (pair ? 2 * G8_BM : G8_BM) + 1;
+  p.n_t = n_t > 0 && pair && !grouped ? n_t : (x_rows - 1) / nt + 1;
   // Dense: tiles of one size, and one copy of their rows a stage; a list's tiles are ragged, their rows come 32 at a time.
   p.nt = grouped ? nt : ((x_rows - 1) / p.n_t + 16) & ~15;
+  if (!grouped) p.n_t = (x_rows - 1) / p.nt + 1;      // (rounded up, they may be fewer)
   p.x_box = grouped ? (nt < 32 ? nt : 32) : (pair ? p.nt / 2 : p.nt);
   p.vec = ((uintptr_t)out & 15) == 0 && ldo % 8 == 0;
   p.vec4 = ((uintptr_t)out & (p.out_f32 ? 15 : 7)) == 0 && ldo % 4 == 0;

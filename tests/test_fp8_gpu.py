@@ -364,3 +364,76 @@ def test_wait_that_runs_out_is_reported(tokens):
         ops.check_tc_error(DEV)
     assert bool((ops.gemm_fp8(x, xs, w, ws, out_dtype=torch.float32) == want).all())
     ops.check_tc_error(DEV)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_products_of_any_sizes(seed):
+    """Sizes that nobody chose, dense and grouped (with tiles of any height): the ways that the estimate picks among."""
+    import random
+    from llm_rs_b200 import ops
+    rng = random.Random(seed)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))
+    T, N, K = log(1, 5000), log(1, 9000), log(1, 9000)
+    while T * N * K > 2e10:
+        T, N, K = (T + 1) // 2, (N + 2) // 3 if N > 3000 else N, (K + 1) // 2
+    x, xs = ops.quantize_fp8(_rows(T, K, seed=seed))
+    w, ws = ops.quantize_fp8(_rows(N, K, seed=seed + 1))
+    xv, wv = _values(x, xs), _values(w, ws)
+    y = ops.gemm_fp8(x, xs, w, ws, out_dtype=torch.float32)
+    assert bool(((y.double() - xv @ wv.t()).abs() <= _bound(xv, wv, torch.float32, K)).all()), (T, N, K)
+    G = min(rng.choice([1, 2, 7, 30]), N)
+    N //= G
+    cuts = sorted(rng.randint(0, T) for _ in range(G - 1))
+    counts = [b - a for a, b in zip([0] + cuts, cuts + [T])]
+    tile_rows = rng.randint(1, 256)
+    tiles, n_tiles, starts = _tiles(counts, tile_rows)
+    out = torch.full((T, N), 7.0, device=DEV)
+    ops.gemm_fp8_grouped(x, xs, w[: G * N].unflatten(0, (G, N)), ws[:, : G * N], out, tiles, n_tiles, tile_rows)
+    for g, (s, n) in enumerate(zip(starts, counts)):
+        wg = wv[g * N: (g + 1) * N]
+        assert bool(((out[s: s + n].double() - xv[s: s + n] @ wg.t()).abs() <= _bound(xv[s: s + n], wg, torch.float32, K)).all()), (T, N, K, G)
+    ops.check_tc_error(DEV)
+
+
+def test_places_past_two_to_the_thirty_one():
+    """Rows, results and streams whose places do not fit 32 bits; the last rows are right."""
+    from llm_rs_b200 import ops
+    K, rows = 4096, 530_000
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = _rows(3, K, spread=False).bfloat16()
+    q, s = ops.quantize_fp8(x)
+    del x
+    tail, tail_s = ops.quantize_fp8(_rows(3, K, spread=False).bfloat16())
+    assert bool((q[-3:].float() == tail.float()).all()) and bool((s[:, -3:].view(torch.uint8) == tail_s.view(torch.uint8)).all())
+    w, ws = ops.quantize_fp8(_rows(100, K, seed=1, spread=False))
+    y = ops.gemm_fp8(q, s, w, ws, out_dtype=torch.float32)
+    assert not bool(y[:-3].any())
+    xv, wv = _values(tail, tail_s), _values(w, ws)
+    assert bool(((y[-3:].double() - xv @ wv.t()).abs() <= _bound(xv, wv, torch.float32, K)).all())
+    del q, s, y
+    x, xs = ops.quantize_fp8(_rows(300_000, 64, seed=2, spread=False))
+    w, ws = ops.quantize_fp8(_rows(8192, 64, seed=3, spread=False))
+    y = ops.gemm_fp8(x, xs, w, ws)
+    for at in (slice(0, 2), slice(262_140, 262_150), slice(299_990, 300_000)):
+        xv, wv = _values(x[at], xs[:, at]), _values(w, ws)
+        assert bool(((y[at].double() - xv @ wv.t()).abs() <= _bound(xv, wv, torch.bfloat16, 64)).all())
+    ops.check_tc_error(DEV)
+
+
+def test_two_streams_at_once():
+    """Products of both kernels, quantised rows between them, in flight on two streams: each as it is alone."""
+    from llm_rs_b200 import ops
+    sets = []
+    for i, (T, N, K) in enumerate(((700, 3000, 2048), (5, 6000, 4096))):
+        sets.append((_rows(T, K, seed=i, spread=False), ops.quantize_fp8(_rows(N, K, seed=i + 5, spread=False))))
+    alone = [ops.gemm_fp8(*ops.quantize_fp8(x), *w, out_dtype=torch.float32) for x, w in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(30):
+        for i, ((x, w), stream) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(ops.gemm_fp8(*ops.quantize_fp8(x), *w, out_dtype=torch.float32))
+    torch.cuda.synchronize()
+    for ys, y in zip(got, alone):
+        assert all(bool((z == y).all()) for z in ys)
+    ops.check_tc_error(DEV)
