@@ -178,8 +178,8 @@ __device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, floa
   return (d < INFINITY ? better : q) * (PLAIN ? u : u + unit.shift);
 }
 
-// `shift`: block = 2^shift, or -1. WAY 0: runs of 16 columns that start on 32-byte boundaries and lie within a run of `block`; 1: fours that do (or the plain
-// layout, block = width); 2: any.
+// `shift`: block = 2^shift, or -1. WAY 0: sixteen columns start on 32-byte boundaries and lie within a run of `block`; 1: four
+// columns lie within one (or the layout is plain, block = width); 2: any.
 template <typename T, int WAY, bool PLAIN>
 __global__ void __launch_bounds__(F8_THREADS)
 f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shift, const GatedUnit unit, const F8Rows o) {
@@ -246,7 +246,8 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
   for (int j = 0; j < 4; ++j)
     if (at + 128 * j + 4 * lane < o.width) {      // (behind the row's end the unit of zeros need not be zero)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * j + i] = at + 128 * j + 4 * lane + i < o.width ? f8_unit<PLAIN>(unit, g[4 * j + i], v[4 * j + i]) : 0.f;
+      for (int i = 0; i < 4; ++i)
+        v[4 * j + i] = at + 128 * j + 4 * lane + i < o.width ? f8_unit<PLAIN>(unit, g[4 * j + i], v[4 * j + i]) : 0.f;
     }
   f8_store_fours(v, q, left, w);
 }
@@ -266,10 +267,10 @@ __device__ __forceinline__ double f8_block_sum(double v, double* red) {
   return t;
 }
 
-// 1 / sqrt(mean + eps), rounded once: CUDA's approximate root and one Newton step in double.
+// 1 / sqrt(mean + eps), rounded once: CUDA's approximate root and one Newton step in double. NaN where the squares pass float32.
 __device__ __forceinline__ float f8_inverse_root(double mean) {
   const double y = rsqrtf((float)mean);
-  return (float)(y * (1.5 - 0.5 * mean * y * y));
+  return y > 0.0 ? (float)(y * (1.5 - 0.5 * mean * y * y)) : NAN;
 }
 
 // Rows of at most 16,384 numbers: a warp keeps the 512 numbers of its word in registers between the sum and the result.

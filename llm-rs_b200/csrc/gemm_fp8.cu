@@ -115,7 +115,9 @@ __device__ __forceinline__ bool g8_wait(uint32_t bar, uint32_t parity, uint32_t 
 __device__ __forceinline__ void g8_prefetch(const CUtensorMap* map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
 }
-__device__ __forceinline__ void g8_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+__device__ __forceinline__ void g8_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 
 // A stage of the ring of copies, or a slot of the ring of scales, and the parity of its barriers' phase.
 struct G8Ring {
@@ -304,7 +306,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   volatile int* sent = abort_flag + 1;      // split: this block's sums have been sent
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t full0 = tc_smem(bars), empty0 = full0 + 8 * C::MAX_STAGES, sc_full0 = empty0 + 8 * C::MAX_STAGES,
-                 sc_empty0 = sc_full0 + 8 * G8_SLOTS, acc_full = sc_empty0 + 8 * G8_SLOTS, received = acc_full + 8, drain_bar = received + 8;
+                 sc_empty0 = sc_full0 + 8 * G8_SLOTS, acc_full = sc_empty0 + 8 * G8_SLOTS, received = acc_full + 8,
+                 drain_bar = received + 8;
   const int kb0 = (int)((long long)split * p.nkb / splits), kb1 = (int)((long long)(split + 1) * p.nkb / splits);
 
   pdl_launch_dependents();
@@ -476,7 +479,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           if (r == split || theirs <= 0) continue;
           asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                        ::"r"(g8_map_rank(tc_smem(sums + (size_t)split * share * G8_BM), (uint32_t)r)),
-                       "r"(tc_smem(own + (size_t)r * share * G8_BM)), "r"((uint32_t)theirs * G8_BM * 4), "r"(g8_map_rank(received, (uint32_t)r))
+                       "r"(tc_smem(own + (size_t)r * share * G8_BM)), "r"((uint32_t)theirs * G8_BM * 4),
+                       "r"(g8_map_rank(received, (uint32_t)r))
                        : "memory");
         }
       }
@@ -488,7 +492,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (!met) g8_cluster_wait();
     if (mine > 0) {
       // The other blocks' sums of this block's tokens: a warp adds up a token's 128 features, four a lane.
-      const bool all = __all_sync(0xffffffffu, g8_wait(received, 0, p.wait_limit, abort_flag));     
+      const bool all = __all_sync(0xffffffffu, g8_wait(received, 0, p.wait_limit, abort_flag));
       const int n = w.f0 + 4 * lane;
       for (int j = warp; j < mine && all; j += G8F_THREADS / 32) {
         const float4* from = reinterpret_cast<const float4*>(sums + (size_t)j * G8_BM) + lane;
@@ -849,8 +853,9 @@ static int g8_device(int* sms) {
 
 typedef void (*G8Kernel)(CUtensorMap, CUtensorMap, G8Params);
 // `allowed`: devices on which the kernel may already use the most shared memory that it takes.
-static int g8_launch(G8Kernel kernel, std::atomic<unsigned long long>* allowed, size_t most, size_t smem, int dev, int threads, dim3 grid, dim3 cluster, const CUtensorMap& mw, const CUtensorMap& mx,
-                     const G8Params& p, cudaStream_t stream) {
+static int g8_launch(G8Kernel kernel, std::atomic<unsigned long long>* allowed, size_t most, size_t smem, int dev, int threads,
+                     dim3 grid, dim3 cluster, const CUtensorMap& mw, const CUtensorMap& mx, const G8Params& p,
+                     cudaStream_t stream) {
   const unsigned long long bit = 1ull << (dev % G8_DEVICES);
   cudaError_t e = cudaSuccess;
   if (dev >= G8_DEVICES || !(allowed->load(std::memory_order_relaxed) & bit)) {
@@ -909,7 +914,8 @@ struct G8Choice { int nt, splits, per_sm, n_t; };
 // The microseconds that each way is expected to take, and the way that takes least. What the parts stand for, fitted to products of
 // 1 to 2,048 tokens on a B200 (16 x 128 x 128 takes 2.9 us):
 //   a block copies, and its MMAs take, a block of k in .18 us + .6 ns a token; the blocks of an SM together get some 138 GB/s, all
-//   together the memory's 6.3 TB/s; a wave of blocks after another starts 2 us late; a split costs .4 us + 35 ns a token of the tile for the exchange of the sums;
+//   together the memory's 6.3 TB/s; a wave of blocks after another starts 2 us late; a split costs .4 us + 35 ns a token of the
+//   tile for the exchange of the sums;
 //   a pair of the other kernel takes .25 us + .72 ns a token for a block of k of its 256 features (the copies; the MMAs of 256
 //   tokens are .27), .2 us a tile more, or .8 where two neighbours do not fit tensor memory together.
 // Measured, us (tokens x features x K; NT / splits): 1 x 6,144 x 4,096 16/1 9.4, 16/2 8.1, 16/5 7.7, 16/8 10.7; 32 x 4,096 x 4,096

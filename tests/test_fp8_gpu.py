@@ -165,6 +165,22 @@ def test_norm(rows, K, dtype):
             assert not bool(picked[0][i].view(torch.uint8).any()) and not bool(picked[1][:, i].view(torch.uint8).any())
 
 
+@pytest.mark.parametrize("K", [512, 515, 17000])
+def test_norm_of_rows_out_of_range(K):
+    """Squares past float32, an infinity, a NaN: that row is NaN, its neighbours are as they are without it."""
+    from llm_rs_b200 import ops
+    h = _rows(6, K, spread=False)
+    w = torch.ones(K, device=DEV)
+    q, s = ops.add_rmsnorm_fp8(h.clone(), None, w, 1e-6)
+    h[0] *= 1e25
+    h[2, K - 1], h[4, 0], h[5] = float("inf"), float("nan"), 0.0
+    q2, s2 = ops.add_rmsnorm_fp8(h, None, w, 1e-6)
+    assert all(bool(q2[r].float().isnan().all()) for r in (0, 4)) and bool(q2[2, K - 1].float().isnan())
+    assert not bool(q2[5].view(torch.uint8).any())
+    for r in (1, 3):
+        assert bool((q2[r].float() == q[r].float()).all()) and bool((s2[:, r].view(torch.uint8) == s[:, r].view(torch.uint8)).all())
+
+
 # -- products ---------------------------------------------------------------------------------------------------------
 def _bound(x, w, out_dtype, K):
     mag = x.abs() @ w.abs().t()
@@ -437,3 +453,19 @@ def test_two_streams_at_once():
     for ys, y in zip(got, alone):
         assert all(bool((z == y).all()) for z in ys)
     ops.check_tc_error(DEV)
+
+
+@pytest.mark.parametrize("nt,splits", [(16, 1), (16, 3), (16, 8), (32, 2), (32, 7), (64, 1), (64, 5), (128, 1), (128, 2), (128, 8), (256, 1)])
+@pytest.mark.parametrize("tokens,features,K", [(1, 130, 1100), (27, 300, 4000), (140, 520, 1024), (300, 1000, 2500)])
+def test_every_way_of_a_product(tokens, features, K, nt, splits):
+    """Tokens a tile and blocks that share a tile's k, whatever the estimate would take for these sizes."""
+    from llm_rs_b200 import ops
+    x, xs = ops.quantize_fp8(_rows(tokens, K, seed=tokens))
+    w, ws = ops.quantize_fp8(_rows(features, K, seed=features + 1))
+    y = torch.empty((tokens, features), device=DEV)
+    ops._check(ops._fp8_product()(
+        x.data_ptr(), x.stride(0), xs.data_ptr(), tokens, tokens, w.data_ptr(), w.stride(0), ws.data_ptr(), features, y.data_ptr(),
+        features, ops.F32, 0, features, K, 1, None, None, 0, 0, nt, splits, ops.tc_error_flag(DEV).data_ptr(), ops._fp8_stream(x)), "gemm_fp8")
+    ops.check_tc_error(DEV)
+    xv, wv = _values(x, xs), _values(w, ws)
+    assert bool(((y.double() - xv @ wv.t()).abs() <= _bound(xv, wv, torch.float32, K)).all())
