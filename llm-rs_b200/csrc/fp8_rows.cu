@@ -72,6 +72,61 @@ __device__ __forceinline__ void f8_store_runs(float (&v)[16], uint8_t* q, uint32
   if ((threadIdx.x & 31) == 0) *word = w;
 }
 
+// Eight consecutive numbers, from a 32-byte (float32) or a 16-byte boundary.
+__device__ __forceinline__ void f8_load8(const float* p, float* v) {
+  uint32_t r[8];
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void f8_load8(const __nv_bfloat16* p, float* v) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  const uint32_t r[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(r[i] << 16);
+    v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void f8_put8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+// The warp's 512 numbers by eights (v[8 h + i] is number 256 h + 8 lane + i); `left` numbers of the row are left, a multiple of 16.
+// The scale's byte grows with the magnitude, so that the bytes of the lanes' own maxima are what is compared: those of both halves
+// in one register.
+__device__ __forceinline__ void f8_store_eights(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
+  const int lane = threadIdx.x & 31;
+  float top[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top[0] = fmaxf(top[0], fabsf(v[i])), top[1] = fmaxf(top[1], fabsf(v[8 + i]));
+  uint32_t both = f8_scale_byte(top[0]) | f8_scale_byte(top[1]) << 16;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (256 * h + 8 * lane >= left) continue;
+    const float inv = f8_inverse(h ? both >> 16 : both & 0xffffu);
+    float* x = v + 8 * h;
+    uint2 p;
+    p.x = f8_pack2(x[0] * inv, x[1] * inv) | f8_pack2(x[2] * inv, x[3] * inv) << 16;
+    p.y = f8_pack2(x[4] * inv, x[5] * inv) | f8_pack2(x[6] * inv, x[7] * inv) << 16;
+    if (isinf(top[h])) {
+      p.x = f8_pack2_any(x[0] * inv, x[1] * inv) | f8_pack2_any(x[2] * inv, x[3] * inv) << 16;
+      p.y = f8_pack2_any(x[4] * inv, x[5] * inv) | f8_pack2_any(x[6] * inv, x[7] * inv) << 16;
+    }
+    *reinterpret_cast<uint2*>(q + 256 * h + 8 * lane) = p;
+  }
+  // Lanes 0-15 hold the bytes of blocks 0 and 2, the others those of 1 and 3.
+  uint32_t w = both << (lane < 16 ? 0 : 8);
+  w |= __shfl_xor_sync(0xffffffffu, w, 16);
+  if (lane == 0) *word = w;
+}
+
 // Four consecutive numbers, of which `n` are there (zeros behind them), from any address. bfloat16 numbers come by the words that hold
 // them: a word's other half lies in the same aligned four bytes as the number that is asked for.
 __device__ __forceinline__ void f8_load4(const float* p, int n, float* v) {
@@ -168,14 +223,14 @@ f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, cons
 // GatedUnit in fewer instructions: the quotient by an approximate reciprocal and one step of the remainder, off by less than an ulp as
 // a division is; PLAIN is silu(gate) * up. What bounds the kernel is these instructions beside the memory: 2,048 rows of 12,288
 // took 33 us with the division, 24.5 with this (19.5 at 6.45 TB/s).
+constexpr float F8_LOG2E = 1.44269504088896f;      // log2(e)
 template <bool PLAIN>
 __device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, float up) {
   const float g = PLAIN ? gate : fminf(gate, unit.limit), u = PLAIN ? up : fminf(fmaxf(up, -unit.limit), unit.limit);
-  const float d = 1.0f + expf(PLAIN ? -g : -unit.alpha * g);
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));      // (0 from 2^126 on: the unit of a gate below -87 is 0)
-  const float q = g * r, better = fmaf(fmaf(-q, d, g), r, q);
-  return (d < INFINITY ? better : q) * (PLAIN ? u : u + unit.shift);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * (PLAIN ? -F8_LOG2E : -F8_LOG2E * unit.alpha)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));      // (0 from 2^126 on: the unit of a gate below -87 is 0)
+  return g * r * (PLAIN ? u : u + unit.shift);
 }
 
 // `shift`: block = 2^shift, or -1. WAY 0: sixteen columns start on 32-byte boundaries and lie within a run of `block`; 1: four
@@ -254,31 +309,34 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
 
 // ---- the residual sum and the norm ------------------------------------------------------------------------------------
 // h += delta, then h / sqrt(mean(h^2) + eps) * weight in 8 bits; with `rows` row i comes from row rows[i] of h and delta, and h is
-// left as it is. A block per row; the sum of squares is made in float32 by each thread and in double over the threads.
-__device__ __forceinline__ double f8_block_sum(double v, double* red) {
+// left as it is. A block per row; sums are float32.
+__device__ __forceinline__ float f8_block_sum(float v, float4* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0) red[warp] = v;
+  float* at = reinterpret_cast<float*>(red);
+  if (lane == 0) at[warp] = v;
+  if (warp == 0 && lane >= n) at[lane] = 0.f;
   __syncthreads();
-  double t = lane < n ? red[lane] : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  float t = 0.f;
+  for (int i = 0; 4 * i < n; ++i) {
+    const float4 r = red[i];
+    t += (r.x + r.y) + (r.z + r.w);
+  }
   return t;
 }
 
-// 1 / sqrt(mean + eps), rounded once: CUDA's approximate root and one Newton step in double. NaN where the squares pass float32.
-__device__ __forceinline__ float f8_inverse_root(double mean) {
-  const double y = rsqrtf((float)mean);
-  return y > 0.0 ? (float)(y * (1.5 - 0.5 * mean * y * y)) : NAN;
+// 1 / sqrt(mean of the squares + eps). NaN where the squares pass float32.
+__device__ __forceinline__ float f8_inverse_root(float squares, int width, float eps) {
+  return squares < INFINITY ? 1.0f / sqrtf(squares / (float)width + eps) : NAN;
 }
 
 // Rows of at most 16,384 numbers: a warp keeps the 512 numbers of its word in registers between the sum and the result.
 template <typename T, bool RUNS, int MOST>
 __global__ void __launch_bounds__(MOST, MOST == 512 ? 3 : 1)
 f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight, const int* __restrict__ rows,
-               int h_rows, float eps, double per, const F8Rows o) {
-  __shared__ double red[32];
+               int h_rows, float eps, const F8Rows o) {
+  __shared__ float4 red[8];
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.x, lane = threadIdx.x & 31, word = threadIdx.x >> 5, from = rows ? rows[r] : r;
@@ -290,20 +348,20 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
   if (RUNS) {
-    if (16 * lane < left) {
-      f8_load16(hr + 16 * lane, v);
-      if (dr) {
-        float d[16];
-        f8_load16(dr + 16 * lane, d);
+    float d[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += d[i];
-        if (!rows) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(hr + 16 * lane + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        }
+    for (int h = 0; h < 2; ++h)
+      if (256 * h + 8 * lane < left) {
+        f8_load8(hr + 256 * h + 8 * lane, v + 8 * h);
+        if (dr) f8_load8(dr + 256 * h + 8 * lane, d + 8 * h);
       }
-    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (dr && 256 * h + 8 * lane < left) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * h + i] += d[8 * h + i];
+        if (!rows) f8_put8(hr + 256 * h + 8 * lane, v + 8 * h);
+      }
   } else {
     float d[16];
     if (left >= F8_WORD) {
@@ -335,12 +393,14 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-  const float inv = f8_inverse_root(f8_block_sum((double)ss, red) * per + (double)eps);
+  const float inv = f8_inverse_root(f8_block_sum(ss, red), o.width, eps);
   float wt[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) wt[i] = 0.f;
   if (RUNS) {
-    if (16 * lane < left) f8_load16(weight + at + 16 * lane, wt);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (256 * h + 8 * lane < left) f8_load8(weight + at + 256 * h + 8 * lane, wt + 8 * h);
   } else {
     if (left >= F8_WORD) {
 #pragma unroll
@@ -354,13 +414,13 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
   const int there = o.width - at;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int c = RUNS ? 16 * lane : 128 * (i / 4) + 4 * lane + i % 4;
+    const int c = RUNS ? 256 * (i / 8) + 8 * lane : 128 * (i / 4) + 4 * lane + i % 4;
     v[i] = c < left ? v[i] * inv * wt[i] : 0.f;      // (inv may be no number)
   }
   uint8_t* q = o.q + (size_t)r * o.pitch + at;
   uint32_t* w = o.words + (size_t)word * o.rows + r;
   if (RUNS)
-    f8_store_runs(v, 16 * lane < there ? q + 16 * lane : nullptr, w);
+    f8_store_eights(v, q, there, w);
   else
     f8_store_fours(v, q, there, w);
 }
@@ -370,8 +430,8 @@ constexpr int F8_NORM_THREADS = 512;
 template <typename T>
 __global__ void __launch_bounds__(F8_NORM_THREADS)
 f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight,
-                     const int* __restrict__ rows, int h_rows, float eps, double per, const F8Rows o) {
-  __shared__ double red[32];
+                     const int* __restrict__ rows, int h_rows, float eps, const F8Rows o) {
+  __shared__ float4 red[8];
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.x, from = rows ? rows[r] : r, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -388,8 +448,8 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
       }
       ss = fmaf(v, v, ss);
     }
-  const double total = f8_block_sum((double)ss, red);      // (its barrier also orders the sums above before the loads below)
-  const float inv = f8_inverse_root(total * per + (double)eps);
+  const float total = f8_block_sum(ss, red);      // (its barrier also orders the sums above before the loads below)
+  const float inv = f8_inverse_root(total, o.width, eps);
   for (int word = warp; word < o.n_words; word += F8_NORM_THREADS / 32) {
     const int at = word * F8_WORD, left = o.width - at;
     float v[16];
@@ -477,16 +537,15 @@ LLMRS_API int llmrs_silu_mul_fp8(const void* gu, int dtype, long long gu_stride,
 template <typename T>
 static cudaError_t f8_launch_norm(float* h, const T* delta, const float* weight, const int* rows, int h_rows, float eps,
                                   const F8Rows& o, cudaStream_t stream) {
-  const double per = 1.0 / o.width;
   if (o.n_words > 32)
     return llmrs_launch(f8_norm_long_kernel<T>, dim3(o.rows), dim3(F8_NORM_THREADS), 0, stream, true, h, delta, weight, rows, h_rows,
-                        eps, per, o);
+                        eps, o);
   const bool runs = f8_in_runs(h, o.width, 4, o.width) && ((uintptr_t)weight & 31) == 0 &&
                     (!delta || f8_in_runs(delta, o.width, (int)sizeof(T), o.width));
   auto* k = o.n_words <= 16 ? (runs ? f8_norm_kernel<T, true, 512> : f8_norm_kernel<T, false, 512>)
                             : (runs ? f8_norm_kernel<T, true, 1024> : f8_norm_kernel<T, false, 1024>);
   return llmrs_launch(k, dim3(o.rows), dim3(o.n_words * 32), 0, stream, true,
-                      h, delta, weight, rows, h_rows, eps, per, o);
+                      h, delta, weight, rows, h_rows, eps, o);
 }
 
 // h [h_rows, width] float32 and delta (or null) of `dtype`, contiguous.
