@@ -1,28 +1,20 @@
 // Rows in 8 bits (fp8.cuh) from rows as they are, from a gated unit, and from a residual sum and its norm: what the products of
 // gemm_fp8.cu read. All three are bound by memory: a number is read once, its byte written once.
 //
-// A warp makes 512 numbers of a row, which is one word of scales. Two ways of dealing the numbers to lanes:
-//   rows that start on 32-byte boundaries   a lane takes 16 consecutive numbers (loads of 32 bytes, a store of 16); a block's
-//                                           maximum is the maximum over 8 neighbouring lanes
-//   all others                              a lane takes 4 consecutive numbers of each of the four blocks (loads of what is
-//                                           aligned, stores of 4 bytes: q's rows start at multiples of 16); a block's maximum is the
-//                                           maximum over the warp
+// A warp makes 512 numbers of a row, which is one word of scales. Three ways of dealing the numbers to lanes (F8Way):
+//   runs    rows of whole sixteens of bfloat16 that start on 32-byte boundaries: a lane takes 16 consecutive numbers (loads of 32 bytes, a
+//           store of 16); a block's maximum is the maximum over 8 neighbouring lanes
+//   fours   rows of whole fours that start on the boundaries of four numbers: 4 consecutive numbers of each of the four blocks
+//           (loads of 16 bytes of float32, of 8 of bfloat16; stores of 4); a block's maximum is the maximum over the warp. The norm
+//           takes this way for aligned rows: its loads and stores of 32 bytes a lane took 41.1 us where those of 16 take 35.5
+//           (4,001 rows of 5,120)
+//   ones    all others: every 32nd number, so that a warp's loads and stores are contiguous whatever the alignment
 #include "fp8.cuh"
 
 constexpr int F8_THREADS = 256;
+enum F8Way : int { F8_RUNS = 0, F8_FOURS = 1, F8_PAIRS = 2, F8_ONES = 3 };
 
 // Sixteen consecutive numbers from a 32-byte boundary.
-__device__ __forceinline__ void f8_load16(const float* p, float (&v)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t r[8];
-    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "l"(p + 8 * h));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(r[i]);
-  }
-}
 __device__ __forceinline__ void f8_load16(const __nv_bfloat16* p, float (&v)[16]) {
   uint32_t r[8];
   asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -72,98 +64,91 @@ __device__ __forceinline__ void f8_store_runs(float (&v)[16], uint8_t* q, uint32
   if ((threadIdx.x & 31) == 0) *word = w;
 }
 
-// Eight consecutive numbers, from a 32-byte (float32) or a 16-byte boundary.
-__device__ __forceinline__ void f8_load8(const float* p, float* v) {
-  uint32_t r[8];
-  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "l"(p));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+// Four consecutive numbers, from a 16-byte (float32) or an 8-byte boundary.
+__device__ __forceinline__ void f8_load4(const float* p, float* v) {
+  const float4 q = *reinterpret_cast<const float4*>(p);
+  v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
 }
-__device__ __forceinline__ void f8_load8(const __nv_bfloat16* p, float* v) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p);
-  const uint32_t r[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(r[i] << 16);
-    v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ void f8_put8(float* p, const float* v) {
-  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
-               "f"(v[5]), "f"(v[6]), "f"(v[7])
-               : "memory");
+__device__ __forceinline__ void f8_load4(const __nv_bfloat16* p, float* v) {
+  const uint2 q = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(q.x << 16), v[1] = __uint_as_float(q.x & 0xffff0000u);
+  v[2] = __uint_as_float(q.y << 16), v[3] = __uint_as_float(q.y & 0xffff0000u);
 }
 
-// The warp's 512 numbers by eights (v[8 h + i] is number 256 h + 8 lane + i); `left` numbers of the row are left, a multiple of 16.
-// The scale's byte grows with the magnitude, so that the bytes of the lanes' own maxima are what is compared: those of both halves
-// in one register.
-__device__ __forceinline__ void f8_store_eights(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
+// This lane's share of a warp's 512 numbers, the first of which is *at(0), by fours or one by one; `left` numbers of the row are left.
+template <int WAY, typename At>
+__device__ __forceinline__ void f8_load(const At& at, int left, float (&v)[16]) {
   const int lane = threadIdx.x & 31;
-  float top[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top[0] = fmaxf(top[0], fabsf(v[i])), top[1] = fmaxf(top[1], fabsf(v[8 + i]));
-  uint32_t both = f8_scale_byte(top[0]) | f8_scale_byte(top[1]) << 16;
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (256 * h + 8 * lane >= left) continue;
-    const float inv = f8_inverse(h ? both >> 16 : both & 0xffffu);
-    float* x = v + 8 * h;
-    uint2 p;
-    p.x = f8_pack2(x[0] * inv, x[1] * inv) | f8_pack2(x[2] * inv, x[3] * inv) << 16;
-    p.y = f8_pack2(x[4] * inv, x[5] * inv) | f8_pack2(x[6] * inv, x[7] * inv) << 16;
-    if (isinf(top[h])) {
-      p.x = f8_pack2_any(x[0] * inv, x[1] * inv) | f8_pack2_any(x[2] * inv, x[3] * inv) << 16;
-      p.y = f8_pack2_any(x[4] * inv, x[5] * inv) | f8_pack2_any(x[6] * inv, x[7] * inv) << 16;
-    }
-    *reinterpret_cast<uint2*>(q + 256 * h + 8 * lane) = p;
+  for (int i = 0; i < 16; i += WAY == F8_FOURS ? 4 : 1) {
+    if (WAY == F8_FOURS && 32 * i + 4 * lane < left) f8_load4(at(32 * i + 4 * lane), v + i);
+    if (WAY == F8_ONES && 32 * i + lane < left) v[i] = to_float(*at(32 * i + lane));
   }
-  // Lanes 0-15 hold the bytes of blocks 0 and 2, the others those of 1 and 3.
-  uint32_t w = both << (lane < 16 ? 0 : 8);
-  w |= __shfl_xor_sync(0xffffffffu, w, 16);
-  if (lane == 0) *word = w;
 }
-
-// Four consecutive numbers, of which `n` are there (zeros behind them), from any address. bfloat16 numbers come by the words that hold
-// them: a word's other half lies in the same aligned four bytes as the number that is asked for.
-__device__ __forceinline__ void f8_load4(const float* p, int n, float* v) {
+// By pairs, from any address: aligned pairs are loaded; where the row starts in the middle of one, a lane's second number is the first
+// of the next lane's.
+__device__ __forceinline__ void f8_load_pairs(const __nv_bfloat16* p, int left, float (&v)[16]) {
+  const int lane = threadIdx.x & 31, odd = (int)((uintptr_t)p >> 1) & 1;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p - odd);
+  uint32_t r[9];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+  for (int i = 0; i < 9; ++i) r[i] = 2 * (32 * i + lane) - odd < left && (i < 8 || lane < odd) ? __ldg(w + 32 * i + lane) : 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (odd) r[i] = __funnelshift_r(r[i], __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1] : r[i], lane + 1), 16);
+    const int n = 64 * i + 2 * lane;
+    v[2 * i] = n < left ? __uint_as_float(r[i] << 16) : 0.f;
+    v[2 * i + 1] = n + 1 < left ? __uint_as_float(r[i] & 0xffff0000u) : 0.f;
+  }
 }
-__device__ __forceinline__ void f8_load4(const __nv_bfloat16* p, int n, float* v) {
-  const uint32_t odd = (uint32_t)((uintptr_t)p >> 1) & 1u;      // the first number is a word's upper half
-  const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)p & ~(uintptr_t)3);
-  if (n >= 4) {
-    const uint32_t a = w[0], b = w[1], c = odd ? w[2] : 0u;
-    const uint32_t lo = __funnelshift_r(a, b, 16 * odd), hi = __funnelshift_r(b, c, 16 * odd);
-    v[0] = __uint_as_float(lo << 16), v[1] = __uint_as_float(lo & 0xffff0000u);
-    v[2] = __uint_as_float(hi << 16), v[3] = __uint_as_float(hi & 0xffff0000u);
-  } else {
+__device__ __forceinline__ void f8_load_pairs(const float* p, int left, float (&v)[16]) {
+  const int lane = threadIdx.x & 31, odd = (int)((uintptr_t)p >> 2) & 1;
+  const float2* w = reinterpret_cast<const float2*>(p - odd);
+  float2 r[9];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+  for (int i = 0; i < 9; ++i) {
+    r[i] = make_float2(0.f, 0.f);
+    if (2 * (32 * i + lane) - odd < left && (i < 8 || lane < odd)) r[i] = __ldg(w + 32 * i + lane);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (odd) r[i] = make_float2(r[i].y, __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1].x : r[i].x, lane + 1));
+    const int n = 64 * i + 2 * lane;
+    v[2 * i] = n < left ? r[i].x : 0.f;
+    v[2 * i + 1] = n + 1 < left ? r[i].y : 0.f;
   }
 }
 
-// The warp's 512 numbers by fours (v[4 j + i] is number 128 j + 4 lane + i); `left` numbers of the row are left. The last word of
-// a row of q is written whole.
-__device__ __forceinline__ void f8_store_fours(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
+// The warp's 512 numbers, of which `left` are there: v[4 j + i] is number 128 j + 4 lane + i (fours), 128 j + 64 (i / 2) + 2 lane + i % 2
+// (pairs), 128 j + 32 i + lane (ones). Room behind a row's end, which reaches to the next multiple of 16, may be written.
+template <int WAY>
+__device__ __forceinline__ void f8_store(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
   const int lane = threadIdx.x & 31;
   uint32_t w = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    float* x = v + 4 * j;
     // The bits of magnitudes are ordered as whole numbers, whose maximum over a warp is one instruction (a NaN counts as 0).
-    const float own = fmaxf(fmaxf(fmaxf(fabsf(v[4 * j]), fabsf(v[4 * j + 1])), fmaxf(fabsf(v[4 * j + 2]), fabsf(v[4 * j + 3]))), 0.f);
+    const float own = fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))), 0.f);
     const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(own)));
     const uint32_t byte = f8_scale_byte(top);
     const float inv = f8_inverse(byte);
     w |= byte << (8 * j);
-    uint32_t p = f8_pack2(v[4 * j] * inv, v[4 * j + 1] * inv) | f8_pack2(v[4 * j + 2] * inv, v[4 * j + 3] * inv) << 16;
-    if (isinf(top))
-      p = f8_pack2_any(v[4 * j] * inv, v[4 * j + 1] * inv) | f8_pack2_any(v[4 * j + 2] * inv, v[4 * j + 3] * inv) << 16;
-    if (128 * j + 4 * lane < left) *reinterpret_cast<uint32_t*>(q + 128 * j + 4 * lane) = p;
+    uint32_t p = f8_pack2(x[0] * inv, x[1] * inv) | f8_pack2(x[2] * inv, x[3] * inv) << 16;
+    if (isinf(top)) p = f8_pack2_any(x[0] * inv, x[1] * inv) | f8_pack2_any(x[2] * inv, x[3] * inv) << 16;
+    if (WAY == F8_FOURS) {
+      if (128 * j + 4 * lane < left) *reinterpret_cast<uint32_t*>(q + 128 * j + 4 * lane) = p;
+    } else if (WAY == F8_PAIRS) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = 128 * j + 64 * h + 2 * lane;
+        if (n < left) *reinterpret_cast<uint16_t*>(q + n) = (uint16_t)(p >> (16 * h));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (128 * j + 32 * i + lane < left) q[128 * j + 32 * i + lane] = (uint8_t)(p >> (8 * i));
+    }
   }
   if (lane == 0) *word = w;
 }
@@ -178,7 +163,7 @@ struct F8Rows {
 // ---- rows as they are ---------------------------------------------------------------------------------------------
 // Row r from row src[r] (or r) of x; a row whose source is none of x's becomes zeros. A warp makes two words of a row, so that
 // the loads of both are in flight (7,211 rows of 4,096 bfloat16 numbers: 16.1 us with one, 15.0 with two; 13.8 at 6.45 TB/s).
-template <typename T, bool RUNS>
+template <typename T, int WAY>
 __global__ void __launch_bounds__(F8_THREADS)
 f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, const int* __restrict__ src, const F8Rows o) {
   pdl_launch_dependents();
@@ -195,15 +180,12 @@ f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, cons
     const int at = (2 * blockIdx.y + h) * F8_WORD, left = live ? o.width - at : 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[h][i] = 0.f;
-    if (RUNS) {
+    if constexpr (WAY == F8_RUNS) {
       if (16 * lane < left) f8_load16(xr + at + 16 * lane, v[h]);
-    } else if (left >= F8_WORD) {      // no branch between the loads: they are in flight together
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f8_load4(xr + at + 128 * j + 4 * lane, 4, v[h] + 4 * j);
+    } else if constexpr (WAY == F8_PAIRS) {
+      f8_load_pairs(xr + at, left, v[h]);
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (128 * j + 4 * lane < left) f8_load4(xr + at + 128 * j + 4 * lane, left - 128 * j - 4 * lane, v[h] + 4 * j);
+      f8_load<WAY>([&](int c) { return xr + at + c; }, left, v[h]);
     }
   }
 #pragma unroll
@@ -212,10 +194,10 @@ f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, cons
     if (left <= 0) break;
     uint8_t* q = o.q + (size_t)r * o.pitch + word * F8_WORD;
     uint32_t* w = o.words + (size_t)word * o.rows + r;
-    if (RUNS)
+    if constexpr (WAY == F8_RUNS)
       f8_store_runs(v[h], 16 * lane < left ? q + 16 * lane : nullptr, w);
     else
-      f8_store_fours(v[h], q, left, w);
+      f8_store<WAY>(v[h], q, left, w);
   }
 }
 
@@ -233,8 +215,7 @@ __device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, floa
   return g * r * (PLAIN ? u : u + unit.shift);
 }
 
-// `shift`: block = 2^shift, or -1. WAY 0: sixteen columns start on 32-byte boundaries and lie within a run of `block`; 1: four
-// columns lie within one (or the layout is plain, block = width); 2: any.
+// `shift`: block = 2^shift, or -1. A lane's sixteen (runs) or four (fours) columns lie within a run of `block`.
 template <typename T, int WAY, bool PLAIN>
 __global__ void __launch_bounds__(F8_THREADS)
 f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shift, const GatedUnit unit, const F8Rows o) {
@@ -248,14 +229,14 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
   uint8_t* q = o.q + (size_t)r * o.pitch + at;
   uint32_t* w = o.words + (size_t)word * o.rows + r;
   const bool whole = block == o.width;
-  float v[16];
+  // The gate of column c; its up is `block` further.
+  auto gate = [&](int c) { return row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block); };
+  float g[16], v[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  if (WAY == 0) {
-    const int c = at + 16 * lane;
+  for (int i = 0; i < 16; ++i) g[i] = v[i] = 0.f;
+  if constexpr (WAY == F8_RUNS) {
     if (16 * lane < left) {
-      float g[16];
-      const T* p = row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block);
+      const T* p = gate(at + 16 * lane);
       f8_load16(p, g);
       f8_load16(p + block, v);
 #pragma unroll
@@ -264,47 +245,19 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
     f8_store_runs(v, 16 * lane < left ? q + 16 * lane : nullptr, w);
     return;
   }
-  float g[16];
-  if (WAY == 1 && left >= F8_WORD) {      // no branch between the loads: they are in flight together
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = at + 128 * j + 4 * lane;
-      const T* p = row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block);
-      f8_load4(p, 4, g + 4 * j);
-      f8_load4(p + block, 4, v + 4 * j);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = f8_unit<PLAIN>(unit, g[i], v[i]);
-    f8_store_fours(v, q, left, w);
-    return;
+  if constexpr (WAY == F8_PAIRS) {
+    f8_load_pairs(row + at, left, g);
+    f8_load_pairs(row + at + block, left, v);
+  } else {
+    f8_load<WAY>([&](int c) { return gate(at + c); }, left, g);
+    f8_load<WAY>([&](int c) { return gate(at + c) + block; }, left, v);
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = at + 128 * j + 4 * lane, n = o.width - c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) g[4 * j + i] = 0.f;
-    if (n <= 0) continue;
-    if (WAY == 1) {
-      const T* p = row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block);
-      f8_load4(p, n, g + 4 * j);
-      f8_load4(p + block, n, v + 4 * j);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < n) {
-          const T* p = row + c + i + (size_t)((c + i) / block) * block;
-          g[4 * j + i] = to_float(p[0]), v[4 * j + i] = to_float(p[block]);
-        }
-    }
+  for (int i = 0; i < 16; ++i) {
+    const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : WAY == F8_PAIRS ? 64 * (i / 2) + 2 * lane + i % 2 : 32 * i + lane;
+    v[i] = c < left ? f8_unit<PLAIN>(unit, g[i], v[i]) : 0.f;      // (the unit of zeros need not be zero)
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (at + 128 * j + 4 * lane < o.width) {      // (behind the row's end the unit of zeros need not be zero)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[4 * j + i] = at + 128 * j + 4 * lane + i < o.width ? f8_unit<PLAIN>(unit, g[4 * j + i], v[4 * j + i]) : 0.f;
-    }
-  f8_store_fours(v, q, left, w);
+  f8_store<WAY>(v, q, left, w);
 }
 
 // ---- the residual sum and the norm ------------------------------------------------------------------------------------
@@ -332,8 +285,8 @@ __device__ __forceinline__ float f8_inverse_root(float squares, int width, float
 }
 
 // Rows of at most 16,384 numbers: a warp keeps the 512 numbers of its word in registers between the sum and the result.
-template <typename T, bool RUNS, int MOST>
-__global__ void __launch_bounds__(MOST, MOST == 512 ? 3 : 1)
+template <typename T, int WAY, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 512 ? 2 : 1)
 f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* __restrict__ weight, const int* __restrict__ rows,
                int h_rows, float eps, const F8Rows o) {
   __shared__ float4 red[8];
@@ -347,82 +300,37 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  if (RUNS) {
-    float d[16];
+  float d[16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (256 * h + 8 * lane < left) {
-        f8_load8(hr + 256 * h + 8 * lane, v + 8 * h);
-        if (dr) f8_load8(dr + 256 * h + 8 * lane, d + 8 * h);
-      }
+  for (int i = 0; i < 16; ++i) d[i] = 0.f;
+  f8_load<WAY>([&](int c) { return hr + c; }, left, v);
+  if (dr) f8_load<WAY>([&](int c) { return dr + c; }, left, d);
+  if (dr) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (dr && 256 * h + 8 * lane < left) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * h + i] += d[8 * h + i];
-        if (!rows) f8_put8(hr + 256 * h + 8 * lane, v + 8 * h);
-      }
-  } else {
-    float d[16];
-    if (left >= F8_WORD) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f8_load4(hr + 128 * j + 4 * lane, 4, v + 4 * j);
-      if (dr) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f8_load4(dr + 128 * j + 4 * lane, 4, d + 4 * j);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = 128 * j + 4 * lane;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[4 * j + i] = 0.f;
-        if (c < left) f8_load4(hr + c, left - c, v + 4 * j);
-        if (dr && c < left) f8_load4(dr + c, left - c, d + 4 * j);
-      }
-    }
-    if (dr) {
+    for (int i = 0; i < 16; ++i) v[i] += d[i];
+    if (!rows) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int c = 128 * (i / 4) + 4 * lane + i % 4;
-        v[i] += d[i];
-        if (!rows && c < left) hr[c] = v[i];
+        if (WAY == F8_ONES && 32 * i + lane < left) hr[32 * i + lane] = v[i];
+        if (WAY == F8_FOURS && i % 4 == 0 && 32 * i + 4 * lane < left)
+          *reinterpret_cast<float4*>(hr + 32 * i + 4 * lane) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       }
     }
   }
+  float wt[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) wt[i] = 0.f;
+  f8_load<WAY>([&](int c) { return weight + at + c; }, left, wt);
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
   const float inv = f8_inverse_root(f8_block_sum(ss, red), o.width, eps);
-  float wt[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) wt[i] = 0.f;
-  if (RUNS) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (256 * h + 8 * lane < left) f8_load8(weight + at + 256 * h + 8 * lane, wt + 8 * h);
-  } else {
-    if (left >= F8_WORD) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f8_load4(weight + at + 128 * j + 4 * lane, 4, wt + 4 * j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (128 * j + 4 * lane < left) f8_load4(weight + at + 128 * j + 4 * lane, left - 128 * j - 4 * lane, wt + 4 * j);
-    }
-  }
-  const int there = o.width - at;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int c = RUNS ? 256 * (i / 8) + 8 * lane : 128 * (i / 4) + 4 * lane + i % 4;
+    const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : 32 * i + lane;
     v[i] = c < left ? v[i] * inv * wt[i] : 0.f;      // (inv may be no number)
   }
-  uint8_t* q = o.q + (size_t)r * o.pitch + at;
-  uint32_t* w = o.words + (size_t)word * o.rows + r;
-  if (RUNS)
-    f8_store_eights(v, q, there, w);
-  else
-    f8_store_fours(v, q, there, w);
+  f8_store<WAY>(v, o.q + (size_t)r * o.pitch + at, o.width - at, o.words + (size_t)word * o.rows + r);
 }
 
 // Longer rows: read again between the two.
@@ -455,7 +363,7 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int c = at + 128 * (i / 4) + 4 * lane + i % 4;
+      const int c = at + 32 * i + lane;
       v[i] = 0.f;
       if (live && c < o.width) {
         v[i] = hr[c];
@@ -463,7 +371,7 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
         v[i] = v[i] * inv * weight[c];
       }
     }
-    f8_store_fours(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);
+    f8_store<F8_ONES>(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);
   }
 }
 
@@ -476,8 +384,10 @@ static int f8_rows_of(F8Rows* o, const char* what, void* q, long long pitch, voi
   LLMRS_REQUIRE(o->n_words <= 65535, "%s: rows of more than %d numbers", what, 65535 * F8_WORD);
   return 0;
 }
-static bool f8_in_runs(const void* x, long long stride, int size, int width) {
-  return width % 16 == 0 && ((uintptr_t)x & 31) == 0 && stride * size % 32 == 0;
+// How rows that are `stride` numbers of `size` bytes apart may be dealt.
+static F8Way f8_way(const void* x, long long stride, int size, int width) {
+  const long long at = (long long)(uintptr_t)x | stride * size;
+  return size == 2 && width % 16 == 0 && at % 32 == 0 ? F8_RUNS : width % 4 == 0 && at % (4 * size) == 0 ? F8_FOURS : F8_PAIRS;
 }
 // Blocks of eight rows and `words` words.
 static dim3 f8_grid(const F8Rows& o, int words) {
@@ -491,10 +401,13 @@ LLMRS_API int llmrs_quantize_fp8(const void* x, int dtype, long long x_stride, i
   if (rows == 0) return 0;
   cudaError_t e;
   if (dtype == LLMRS_F32) {
-    auto* k = f8_in_runs(x, x_stride, 4, width) ? f8_quantize_kernel<float, true> : f8_quantize_kernel<float, false>;
+    auto* k = f8_way(x, x_stride, 4, width) == F8_FOURS ? f8_quantize_kernel<float, F8_FOURS> : f8_quantize_kernel<float, F8_PAIRS>;
     e = llmrs_launch(k, f8_grid(o, 2), dim3(F8_THREADS), 0, stream, true, (const float*)x, x_stride, x_rows, src, o);
   } else if (dtype == LLMRS_BF16) {
-    auto* k = f8_in_runs(x, x_stride, 2, width) ? f8_quantize_kernel<__nv_bfloat16, true> : f8_quantize_kernel<__nv_bfloat16, false>;
+    const F8Way way = f8_way(x, x_stride, 2, width);
+    auto* k = way == F8_RUNS    ? f8_quantize_kernel<__nv_bfloat16, F8_RUNS>
+              : way == F8_FOURS ? f8_quantize_kernel<__nv_bfloat16, F8_FOURS>
+                                : f8_quantize_kernel<__nv_bfloat16, F8_PAIRS>;
     e = llmrs_launch(k, f8_grid(o, 2), dim3(F8_THREADS), 0, stream, true, (const __nv_bfloat16*)x, x_stride, x_rows, src, o);
   } else {
     return llmrs_fail("quantize_fp8: unknown dtype %d", dtype);
@@ -508,10 +421,14 @@ static cudaError_t f8_launch_unit(const T* gu, long long gu_stride, int block, c
                                   cudaStream_t stream) {
   const bool plain = unit.limit == INFINITY && unit.alpha == 1.0f && unit.shift == 0.0f;
   const int shift = block & (block - 1) ? -1 : __builtin_ctz((unsigned)block);
-  const int way = block % 16 == 0 && f8_in_runs(gu, gu_stride, (int)sizeof(T), o.width) ? 0 : block == o.width || block % 4 == 0 ? 1 : 2;
-  auto* k = way == 0   ? (plain ? f8_unit_kernel<T, 0, true> : f8_unit_kernel<T, 0, false>)
-            : way == 1 ? (plain ? f8_unit_kernel<T, 1, true> : f8_unit_kernel<T, 1, false>)
-                       : (plain ? f8_unit_kernel<T, 2, true> : f8_unit_kernel<T, 2, false>);
+  F8Way way = f8_way(gu, gu_stride, (int)sizeof(T), o.width);
+  if (way == F8_RUNS && block % 16) way = F8_FOURS;
+  if ((way == F8_FOURS && block % 4) || (way == F8_PAIRS && block != o.width)) way = F8_ONES;
+  auto* k = way == F8_FOURS   ? (plain ? f8_unit_kernel<T, F8_FOURS, true> : f8_unit_kernel<T, F8_FOURS, false>)
+            : way == F8_PAIRS ? (plain ? f8_unit_kernel<T, F8_PAIRS, true> : f8_unit_kernel<T, F8_PAIRS, false>)
+                              : (plain ? f8_unit_kernel<T, F8_ONES, true> : f8_unit_kernel<T, F8_ONES, false>);
+  if constexpr (sizeof(T) == 2)
+    if (way == F8_RUNS) k = plain ? f8_unit_kernel<T, F8_RUNS, true> : f8_unit_kernel<T, F8_RUNS, false>;
   return llmrs_launch(k, f8_grid(o, 1), dim3(F8_THREADS), 0, stream, true, gu, gu_stride, block, shift, unit, o);
 }
 
@@ -540,10 +457,10 @@ static cudaError_t f8_launch_norm(float* h, const T* delta, const float* weight,
   if (o.n_words > 32)
     return llmrs_launch(f8_norm_long_kernel<T>, dim3(o.rows), dim3(F8_NORM_THREADS), 0, stream, true, h, delta, weight, rows, h_rows,
                         eps, o);
-  const bool runs = f8_in_runs(h, o.width, 4, o.width) && ((uintptr_t)weight & 31) == 0 &&
-                    (!delta || f8_in_runs(delta, o.width, (int)sizeof(T), o.width));
-  auto* k = o.n_words <= 16 ? (runs ? f8_norm_kernel<T, true, 512> : f8_norm_kernel<T, false, 512>)
-                            : (runs ? f8_norm_kernel<T, true, 1024> : f8_norm_kernel<T, false, 1024>);
+  const bool fours = f8_way(h, o.width, 4, o.width) != F8_PAIRS && ((uintptr_t)weight & 15) == 0 &&
+                     (!delta || f8_way(delta, o.width, (int)sizeof(T), o.width) != F8_PAIRS);
+  auto* k = o.n_words <= 16 ? (fours ? f8_norm_kernel<T, F8_FOURS, 512> : f8_norm_kernel<T, F8_ONES, 512>)
+                            : (fours ? f8_norm_kernel<T, F8_FOURS, 1024> : f8_norm_kernel<T, F8_ONES, 1024>);
   return llmrs_launch(k, dim3(o.rows), dim3(o.n_words * 32), 0, stream, true,
                       h, delta, weight, rows, h_rows, eps, o);
 }
