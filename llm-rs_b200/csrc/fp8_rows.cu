@@ -1,14 +1,18 @@
 // Rows in 8 bits (fp8.cuh) from rows as they are, from a gated unit, and from a residual sum and its norm: what the products of
 // gemm_fp8.cu read. All three are bound by memory: a number is read once, its byte written once.
 //
-// A warp makes 512 numbers of a row, which is one word of scales. Three ways of dealing the numbers to lanes (F8Way):
-//   runs    rows of whole sixteens of bfloat16 that start on 32-byte boundaries: a lane takes 16 consecutive numbers (loads of 32 bytes, a
-//           store of 16); a block's maximum is the maximum over 8 neighbouring lanes
+// A warp makes 512 numbers of a row, which is one word of scales. Four ways of dealing the numbers to lanes (F8Way):
+//   runs    rows of whole sixteens of bfloat16 that start on 32-byte boundaries: a lane takes 16 consecutive numbers (loads of 32
+//           bytes, a store of 16); a block's maximum is the maximum over 8 neighbouring lanes
 //   fours   rows of whole fours that start on the boundaries of four numbers: 4 consecutive numbers of each of the four blocks
-//           (loads of 16 bytes of float32, of 8 of bfloat16; stores of 4); a block's maximum is the maximum over the warp. The norm
-//           takes this way for aligned rows: its loads and stores of 32 bytes a lane took 41.1 us where those of 16 take 35.5
-//           (4,001 rows of 5,120)
-//   ones    all others: every 32nd number, so that a warp's loads and stores are contiguous whatever the alignment
+//           (loads of 16 bytes of float32, of 8 of bfloat16; stores of 4); a block's maximum is the maximum over the warp. float32
+//           goes this way: a norm's loads and stores of 32 bytes a lane took 41.1 us, those of 16 35.3 (4,001 rows of 5,120), a
+//           float32 unit 21.7 and 18.3 (3,000 rows of 4,112)
+//   pairs   all other rows: aligned pairs, 32 neighbours a load, moved over by a number where the row starts inside one. Rows of
+//           4,095 bfloat16 numbers (8,000 of them) took 25.9 us by unaligned fours, 36 one by one, 20.9 so (15.3 at 6.45 TB/s)
+//   ones    every 32nd number: the norm of such rows, whose sums go back where the numbers came from (2,000 rows of 5,001: 32.3 us by
+//           unaligned fours, 23.7 so), and units whose columns alternate by a number that is not a multiple of four
+// Words that lie whole within a row go without a comparison a number: on odd rows the instructions are what bounds.
 #include "fp8.cuh"
 
 constexpr int F8_THREADS = 256;
@@ -75,32 +79,39 @@ __device__ __forceinline__ void f8_load4(const __nv_bfloat16* p, float* v) {
   v[2] = __uint_as_float(q.y << 16), v[3] = __uint_as_float(q.y & 0xffff0000u);
 }
 
-// This lane's share of a warp's 512 numbers, the first of which is *at(0), by fours or one by one; `left` numbers of the row are left.
-template <int WAY, typename At>
+// This lane's share of a warp's 512 numbers, the first of which is *at(0), by fours or one by one; `left` numbers of the row are left
+// (FULL: all of them, which saves a comparison a number).
+template <int WAY, bool FULL, typename At>
 __device__ __forceinline__ void f8_load(const At& at, int left, float (&v)[16]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 16; i += WAY == F8_FOURS ? 4 : 1) {
-    if (WAY == F8_FOURS && 32 * i + 4 * lane < left) f8_load4(at(32 * i + 4 * lane), v + i);
-    if (WAY == F8_ONES && 32 * i + lane < left) v[i] = to_float(*at(32 * i + lane));
+    if (WAY == F8_FOURS && (FULL || 32 * i + 4 * lane < left)) f8_load4(at(32 * i + 4 * lane), v + i);
+    if (WAY == F8_ONES && (FULL || 32 * i + lane < left)) v[i] = to_float(*at(32 * i + lane));
   }
 }
 // By pairs, from any address: aligned pairs are loaded; where the row starts in the middle of one, a lane's second number is the first
 // of the next lane's.
+template <bool FULL>
 __device__ __forceinline__ void f8_load_pairs(const __nv_bfloat16* p, int left, float (&v)[16]) {
   const int lane = threadIdx.x & 31, odd = (int)((uintptr_t)p >> 1) & 1;
   const uint32_t* w = reinterpret_cast<const uint32_t*>(p - odd);
   uint32_t r[9];
 #pragma unroll
-  for (int i = 0; i < 9; ++i) r[i] = 2 * (32 * i + lane) - odd < left && (i < 8 || lane < odd) ? __ldg(w + 32 * i + lane) : 0u;
+  for (int i = 0; i < 9; ++i)
+    r[i] = (FULL || 2 * (32 * i + lane) - odd < left) && (i < 8 || lane < odd) ? __ldg(w + 32 * i + lane) : 0u;
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __funnelshift_r(r[i], __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1] : r[i], lane + 1), 16);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (odd) r[i] = __funnelshift_r(r[i], __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1] : r[i], lane + 1), 16);
     const int n = 64 * i + 2 * lane;
-    v[2 * i] = n < left ? __uint_as_float(r[i] << 16) : 0.f;
-    v[2 * i + 1] = n + 1 < left ? __uint_as_float(r[i] & 0xffff0000u) : 0.f;
+    v[2 * i] = FULL || n < left ? __uint_as_float(r[i] << 16) : 0.f;
+    v[2 * i + 1] = FULL || n + 1 < left ? __uint_as_float(r[i] & 0xffff0000u) : 0.f;
   }
 }
+template <bool FULL>
 __device__ __forceinline__ void f8_load_pairs(const float* p, int left, float (&v)[16]) {
   const int lane = threadIdx.x & 31, odd = (int)((uintptr_t)p >> 2) & 1;
   const float2* w = reinterpret_cast<const float2*>(p - odd);
@@ -108,20 +119,23 @@ __device__ __forceinline__ void f8_load_pairs(const float* p, int left, float (&
 #pragma unroll
   for (int i = 0; i < 9; ++i) {
     r[i] = make_float2(0.f, 0.f);
-    if (2 * (32 * i + lane) - odd < left && (i < 8 || lane < odd)) r[i] = __ldg(w + 32 * i + lane);
+    if ((FULL || 2 * (32 * i + lane) - odd < left) && (i < 8 || lane < odd)) r[i] = __ldg(w + 32 * i + lane);
+  }
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = make_float2(r[i].y, __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1].x : r[i].x, lane + 1));
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (odd) r[i] = make_float2(r[i].y, __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1].x : r[i].x, lane + 1));
     const int n = 64 * i + 2 * lane;
-    v[2 * i] = n < left ? r[i].x : 0.f;
-    v[2 * i + 1] = n + 1 < left ? r[i].y : 0.f;
+    v[2 * i] = FULL || n < left ? r[i].x : 0.f;
+    v[2 * i + 1] = FULL || n + 1 < left ? r[i].y : 0.f;
   }
 }
 
 // The warp's 512 numbers, of which `left` are there: v[4 j + i] is number 128 j + 4 lane + i (fours), 128 j + 64 (i / 2) + 2 lane + i % 2
 // (pairs), 128 j + 32 i + lane (ones). Room behind a row's end, which reaches to the next multiple of 16, may be written.
-template <int WAY>
+template <int WAY, bool FULL>
 __device__ __forceinline__ void f8_store(float (&v)[16], uint8_t* q, int left, uint32_t* word) {
   const int lane = threadIdx.x & 31;
   uint32_t w = 0;
@@ -137,17 +151,17 @@ __device__ __forceinline__ void f8_store(float (&v)[16], uint8_t* q, int left, u
     uint32_t p = f8_pack2(x[0] * inv, x[1] * inv) | f8_pack2(x[2] * inv, x[3] * inv) << 16;
     if (isinf(top)) p = f8_pack2_any(x[0] * inv, x[1] * inv) | f8_pack2_any(x[2] * inv, x[3] * inv) << 16;
     if (WAY == F8_FOURS) {
-      if (128 * j + 4 * lane < left) *reinterpret_cast<uint32_t*>(q + 128 * j + 4 * lane) = p;
+      if (FULL || 128 * j + 4 * lane < left) *reinterpret_cast<uint32_t*>(q + 128 * j + 4 * lane) = p;
     } else if (WAY == F8_PAIRS) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int n = 128 * j + 64 * h + 2 * lane;
-        if (n < left) *reinterpret_cast<uint16_t*>(q + n) = (uint16_t)(p >> (16 * h));
+        if (FULL || n < left) *reinterpret_cast<uint16_t*>(q + n) = (uint16_t)(p >> (16 * h));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (128 * j + 32 * i + lane < left) q[128 * j + 32 * i + lane] = (uint8_t)(p >> (8 * i));
+        if (FULL || 128 * j + 32 * i + lane < left) q[128 * j + 32 * i + lane] = (uint8_t)(p >> (8 * i));
     }
   }
   if (lane == 0) *word = w;
@@ -161,43 +175,56 @@ struct F8Rows {
 };
 
 // ---- rows as they are ---------------------------------------------------------------------------------------------
-// Row r from row src[r] (or r) of x; a row whose source is none of x's becomes zeros. A warp makes two words of a row, so that
-// the loads of both are in flight (7,211 rows of 4,096 bfloat16 numbers: 16.1 us with one, 15.0 with two; 13.8 at 6.45 TB/s).
+// Row r from row src[r] (or r) of x; a row whose source is none of x's becomes zeros. By runs a warp makes two words of a row, so that
+// the loads of both are in flight (7,211 rows of 4,096 bfloat16 numbers: 16.1 us with one, 15.0 with two; 13.8 at 6.45 TB/s). The other
+// ways are bound by their instructions.
+template <typename T, int WAY, bool FULL>
+__device__ __forceinline__ void f8_quantize_word(const T* x, int left, uint8_t* q, int q_left, uint32_t* word) {
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  if constexpr (WAY == F8_PAIRS)
+    f8_load_pairs<FULL>(x, left, v);
+  else
+    f8_load<WAY, FULL>([&](int c) { return x + c; }, left, v);
+  f8_store<WAY, FULL>(v, q, q_left, word);
+}
+
 template <typename T, int WAY>
 __global__ void __launch_bounds__(F8_THREADS)
 f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, const int* __restrict__ src, const F8Rows o) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int r = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5);      // a block: two words of eight rows
+  const int r = blockIdx.x * (F8_THREADS / 32) + (threadIdx.x >> 5);      // a block: a word, or two, of eight rows
   if (r >= o.rows) return;
   const int from = src ? src[r] : r;
   const bool live = from >= 0 && from < x_rows;
   const T* xr = x + (live ? (size_t)from * x_stride : 0);
-  float v[2][16];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int at = (2 * blockIdx.y + h) * F8_WORD, left = live ? o.width - at : 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[h][i] = 0.f;
-    if constexpr (WAY == F8_RUNS) {
-      if (16 * lane < left) f8_load16(xr + at + 16 * lane, v[h]);
-    } else if constexpr (WAY == F8_PAIRS) {
-      f8_load_pairs(xr + at, left, v[h]);
-    } else {
-      f8_load<WAY>([&](int c) { return xr + at + c; }, left, v[h]);
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int word = 2 * blockIdx.y + h, left = o.width - word * F8_WORD;
-    if (left <= 0) break;
-    uint8_t* q = o.q + (size_t)r * o.pitch + word * F8_WORD;
-    uint32_t* w = o.words + (size_t)word * o.rows + r;
-    if constexpr (WAY == F8_RUNS)
-      f8_store_runs(v[h], 16 * lane < left ? q + 16 * lane : nullptr, w);
+  if constexpr (WAY != F8_RUNS) {
+    const int at = blockIdx.y * F8_WORD, q_left = o.width - at;
+    uint8_t* q = o.q + (size_t)r * o.pitch + at;
+    uint32_t* w = o.words + (size_t)blockIdx.y * o.rows + r;
+    if (live && q_left >= F8_WORD)
+      f8_quantize_word<T, WAY, true>(xr + at, q_left, q, q_left, w);
     else
-      f8_store<WAY>(v[h], q, left, w);
+      f8_quantize_word<T, WAY, false>(xr + at, live ? q_left : 0, q, q_left, w);
+  } else {
+    float v[2][16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = (2 * blockIdx.y + h) * F8_WORD, left = live ? o.width - at : 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[h][i] = 0.f;
+      if (16 * lane < left) f8_load16(xr + at + 16 * lane, v[h]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int word = 2 * blockIdx.y + h, left = o.width - word * F8_WORD;
+      if (left <= 0) break;
+      uint8_t* q = o.q + (size_t)r * o.pitch + word * F8_WORD + 16 * lane;
+      f8_store_runs(v[h], 16 * lane < left ? q : nullptr, o.words + (size_t)word * o.rows + r);
+    }
   }
 }
 
@@ -215,7 +242,31 @@ __device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, floa
   return g * r * (PLAIN ? u : u + unit.shift);
 }
 
-// `shift`: block = 2^shift, or -1. A lane's sixteen (runs) or four (fours) columns lie within a run of `block`.
+// gate(c): where column c's gate is; its up is `block` further. A lane's sixteen (runs) or four (fours) columns lie within a run of
+// `block`; pairs: the layout is plain.
+template <typename T, int WAY, bool PLAIN, bool FULL, typename Gate>
+__device__ __forceinline__ void f8_unit_word(const Gate& gate, int block, int at, int left, const GatedUnit& unit, uint8_t* q,
+                                             uint32_t* word) {
+  const int lane = threadIdx.x & 31;
+  float g[16], v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) g[i] = v[i] = 0.f;
+  if constexpr (WAY == F8_PAIRS) {
+    f8_load_pairs<FULL>(gate(at), left, g);
+    f8_load_pairs<FULL>(gate(at) + block, left, v);
+  } else {
+    f8_load<WAY, FULL>([&](int c) { return gate(at + c); }, left, g);
+    f8_load<WAY, FULL>([&](int c) { return gate(at + c) + block; }, left, v);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : WAY == F8_PAIRS ? 64 * (i / 2) + 2 * lane + i % 2 : 32 * i + lane;
+    v[i] = FULL || c < left ? f8_unit<PLAIN>(unit, g[i], v[i]) : 0.f;      // (the unit of zeros need not be zero)
+  }
+  f8_store<WAY, FULL>(v, q, left, word);
+}
+
+// `shift`: block = 2^shift, or -1.
 template <typename T, int WAY, bool PLAIN>
 __global__ void __launch_bounds__(F8_THREADS)
 f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shift, const GatedUnit unit, const F8Rows o) {
@@ -229,13 +280,13 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
   uint8_t* q = o.q + (size_t)r * o.pitch + at;
   uint32_t* w = o.words + (size_t)word * o.rows + r;
   const bool whole = block == o.width;
-  // The gate of column c; its up is `block` further.
   auto gate = [&](int c) { return row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block); };
-  float g[16], v[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) g[i] = v[i] = 0.f;
   if constexpr (WAY == F8_RUNS) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
     if (16 * lane < left) {
+      float g[16];
       const T* p = gate(at + 16 * lane);
       f8_load16(p, g);
       f8_load16(p + block, v);
@@ -243,21 +294,11 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
       for (int i = 0; i < 16; ++i) v[i] = f8_unit<PLAIN>(unit, g[i], v[i]);
     }
     f8_store_runs(v, 16 * lane < left ? q + 16 * lane : nullptr, w);
-    return;
-  }
-  if constexpr (WAY == F8_PAIRS) {
-    f8_load_pairs(row + at, left, g);
-    f8_load_pairs(row + at + block, left, v);
+  } else if (left >= F8_WORD) {
+    f8_unit_word<T, WAY, PLAIN, true>(gate, block, at, left, unit, q, w);
   } else {
-    f8_load<WAY>([&](int c) { return gate(at + c); }, left, g);
-    f8_load<WAY>([&](int c) { return gate(at + c) + block; }, left, v);
+    f8_unit_word<T, WAY, PLAIN, false>(gate, block, at, left, unit, q, w);
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : WAY == F8_PAIRS ? 64 * (i / 2) + 2 * lane + i % 2 : 32 * i + lane;
-    v[i] = c < left ? f8_unit<PLAIN>(unit, g[i], v[i]) : 0.f;      // (the unit of zeros need not be zero)
-  }
-  f8_store<WAY>(v, q, left, w);
 }
 
 // ---- the residual sum and the norm ------------------------------------------------------------------------------------
@@ -303,8 +344,8 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
   float d[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) d[i] = 0.f;
-  f8_load<WAY>([&](int c) { return hr + c; }, left, v);
-  if (dr) f8_load<WAY>([&](int c) { return dr + c; }, left, d);
+  f8_load<WAY, false>([&](int c) { return hr + c; }, left, v);
+  if (dr) f8_load<WAY, false>([&](int c) { return dr + c; }, left, d);
   if (dr) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] += d[i];
@@ -320,7 +361,7 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
   float wt[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) wt[i] = 0.f;
-  f8_load<WAY>([&](int c) { return weight + at + c; }, left, wt);
+  f8_load<WAY, false>([&](int c) { return weight + at + c; }, left, wt);
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
@@ -330,7 +371,7 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
     const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : 32 * i + lane;
     v[i] = c < left ? v[i] * inv * wt[i] : 0.f;      // (inv may be no number)
   }
-  f8_store<WAY>(v, o.q + (size_t)r * o.pitch + at, o.width - at, o.words + (size_t)word * o.rows + r);
+  f8_store<WAY, false>(v, o.q + (size_t)r * o.pitch + at, o.width - at, o.words + (size_t)word * o.rows + r);
 }
 
 // Longer rows: read again between the two.
@@ -371,7 +412,7 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
         v[i] = v[i] * inv * weight[c];
       }
     }
-    f8_store<F8_ONES>(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);
+    f8_store<F8_ONES, false>(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);
   }
 }
 
@@ -402,13 +443,13 @@ LLMRS_API int llmrs_quantize_fp8(const void* x, int dtype, long long x_stride, i
   cudaError_t e;
   if (dtype == LLMRS_F32) {
     auto* k = f8_way(x, x_stride, 4, width) == F8_FOURS ? f8_quantize_kernel<float, F8_FOURS> : f8_quantize_kernel<float, F8_PAIRS>;
-    e = llmrs_launch(k, f8_grid(o, 2), dim3(F8_THREADS), 0, stream, true, (const float*)x, x_stride, x_rows, src, o);
+    e = llmrs_launch(k, f8_grid(o, 1), dim3(F8_THREADS), 0, stream, true, (const float*)x, x_stride, x_rows, src, o);
   } else if (dtype == LLMRS_BF16) {
     const F8Way way = f8_way(x, x_stride, 2, width);
     auto* k = way == F8_RUNS    ? f8_quantize_kernel<__nv_bfloat16, F8_RUNS>
               : way == F8_FOURS ? f8_quantize_kernel<__nv_bfloat16, F8_FOURS>
                                 : f8_quantize_kernel<__nv_bfloat16, F8_PAIRS>;
-    e = llmrs_launch(k, f8_grid(o, 2), dim3(F8_THREADS), 0, stream, true, (const __nv_bfloat16*)x, x_stride, x_rows, src, o);
+    e = llmrs_launch(k, f8_grid(o, way == F8_RUNS ? 2 : 1), dim3(F8_THREADS), 0, stream, true, (const __nv_bfloat16*)x, x_stride, x_rows, src, o);
   } else {
     return llmrs_fail("quantize_fp8: unknown dtype %d", dtype);
   }
