@@ -330,6 +330,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   __syncthreads();
   if (splits > 1) g8_cluster_arrive();
   pdl_wait();      // everything below reads or writes what earlier kernels may have touched
+  const int n_row_tiles = p.tiles ? min(*p.n_tiles, p.max_tiles) : p.n_t;
+  if (blockIdx.x >= (long long)n_row_tiles * p.n_f) {      // a list's tiles may be fewer than the grid has room for; the whole cluster
+    if (splits > 1) g8_cluster_wait();
+    return;
+  }
   // Tensor memory is asked for after the wait: a block that held some while it waits for an earlier kernel could keep that kernel's
   // blocks from theirs. The copies start meanwhile.
   uint32_t tmem_base = 0;
@@ -345,9 +350,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   }
   const uint32_t tmem_scales = tmem_base + C::ACC_COLS;
-  const int n_row_tiles = p.tiles ? min(*p.n_tiles, p.max_tiles) : p.n_t;
-  const bool live = blockIdx.x < (long long)n_row_tiles * p.n_f;      // (a list's tiles may be fewer than the grid has room for)
-  const G8Tile w = live ? g8_tile(p, blockIdx.x, n_row_tiles, G8_BM) : G8Tile{0, 0, 0, 0};
+  const G8Tile w = g8_tile(p, blockIdx.x, n_row_tiles, G8_BM);
   const int w_row = w.group * p.N + w.f0;
   int copies = 0;      // warp 0: stages whose copies it has requested
   // Split: the split-th share of the tile's tokens is this block's to add up.
@@ -355,7 +358,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   bool met = false;
   if (splits > 1 && tid == 0) mbar_expect_tx(received, (uint32_t)((splits - 1) * mine) * G8_BM * 4);      // from the other blocks
 
-  if (!live || w.rows == 0) {
+  if (w.rows == 0) {
     // nothing to compute
   } else if (warp == 0) {
     if (tc_elect_one()) {
@@ -908,67 +911,73 @@ static int g8_launch_few(const CUtensorMap& mw, const CUtensorMap& mx, G8Params&
                    dim3((unsigned)tiles, 1, (unsigned)splits), dim3(1, 1, (unsigned)splits), mw, mx, p, stream);
 }
 
+// Blocks of the few-token kernel an SM: two where one each would not hold them all (clusters leave SMs over).
+static int g8_per_sm(long long blocks, int splits, int sms) { return blocks > (splits > 2 ? sms * 4 / 5 : sms) ? 2 : 1; }
+
 // The way of a product: tokens a tile (256: on pairs), blocks that share a tile's k, blocks an SM, tiles of tokens (pairs, dense).
 struct G8Choice { int nt, splits, per_sm, n_t; };
 
-// The microseconds that each way is expected to take, and the way that takes least. What the parts stand for, fitted to products of
-// 1 to 2,048 tokens on a B200 (16 x 128 x 128 takes 2.9 us):
-//   a block copies, and its MMAs take, a block of k in .18 us + .6 ns a token; the blocks of an SM together get some 138 GB/s, all
-//   together the memory's 6.3 TB/s; a wave of blocks after another starts 2 us late; a split costs .4 us + 35 ns a token of the
-//   tile for the exchange of the sums;
-//   a pair of the other kernel takes .25 us + .72 ns a token for a block of k of its 256 features (the copies; the MMAs of 256
-//   tokens are .27), .2 us a tile more, or .8 where two neighbours do not fit tensor memory together.
+// The microseconds that each way is expected to take, and the way that takes least. What the parts stand for, fitted to some 5,900
+// products of 1 to 16,384 rows, dense and of 4 to 64 groups, each timed every way on a B200 (over 2,700 others the way taken is on
+// average 2 % behind the best one, in one of a hundred more than 30 %; 16 x 128 x 128 takes 2.9 us):
+//   a block copies, and its MMAs take, a block of k in .10 us + .6 ns a token; the blocks of an SM together get some 120 GB/s, all
+//   together 10 TB/s (the memory and the L2); a wave of blocks after another starts 2.7 us late, or .5 where the memory is what
+//   bounds; a split costs .56 us + 27 ns a token for the exchange of the sums; a wave of a list's blocks that have no tile .13 us;
+//   a pair of the other kernel takes .257 us + .45 ns a token for a block of k of its 256 features (the copies; the MMAs of 256
+//   tokens are .27), .8 us a tile more, or 1 where two neighbours do not fit tensor memory together.
 // Measured, us (tokens x features x K; NT / splits): 1 x 6,144 x 4,096 16/1 9.4, 16/2 8.1, 16/5 7.7, 16/8 10.7; 32 x 4,096 x 4,096
 // 32/1 8.8, 32/3 7.2, 16/4 7.7; 128 x 6,144 x 4,096 64/1 10.3, 64/2 12.4, 128/1 11.8, pair 17.5; 512 x 4,096 x 4,096 128/1 11.8, 64/1
-// 14.1, pair 17.4; 2,048 x 4,096 x 4,096 pair 31.0, 128/1 37.2.
-// tile_rows 0: dense, n_t is found here; else the most rows of a list's tiles, of which there are at most n_t.
-static G8Choice g8_choose(int rows, int tile_rows, int n_t, int N, int K, long long weight_rows, int sms) {
-  const int nkb = (K - 1) / G8_BK + 1;
-  const double memory = ((double)weight_rows + rows) * K / 6.3e6;
+// 14.1, pair 17.4; 2,048 x 4,096 x 4,096 pair 31.0, 128/1 37.2; 128 rows of 32 groups of 2,048 x 2,048 32/1 22.4, pair 28.6.
+// tile_rows 0: dense; else the most rows of a list's tiles, of which there are at most `max_tiles`, and no more than rows as a rule.
+static G8Choice g8_choose(int rows, int tile_rows, int max_tiles, int groups, int N, int K, int sms) {
+  const int nkb = (K - 1) / G8_BK + 1, live = max_tiles < rows ? max_tiles : rows;
+  const int fill = tile_rows ? (rows - 1) / live + 1 : 0;      // rows a tile has on average
+  const double memory = ((double)(groups < rows ? groups : rows) * N + rows) * K / 10e6;
   G8Choice best = {256, 1, 1, 0};
   const int pairs = sms / 2 > 0 ? sms / 2 : 1, pair_f = (N - 1) / 256 + 1;
   double least = 1e30;
-  const int from = tile_rows ? n_t : (rows - 1) / 256 + 1, to = tile_rows ? n_t : (rows - 1) / 128 + 1;
+  const int from = tile_rows ? live : (rows - 1) / 256 + 1, to = tile_rows ? live : (rows - 1) / 128 + 1;
   for (int tiles = from; tiles <= to; ++tiles) {      // (more than a few are not tried: the first ones differ most)
     if (tiles > from + 8) break;
-    const int n = tile_rows ? tile_rows : ((rows - 1) / tiles + 16) & ~15;
-    const double waves = (double)(((long long)tiles * pair_f + pairs - 1) / pairs), step = .25 + .00072 * n;
-    const double walk = waves * (nkb * step + (2 * n > G8P_SUM_COLS ? .8 : .2));
-    const double t = 5.0 + (walk > memory ? walk : memory);
+    int n = ((rows - 1) / tiles + 16) & ~15;
+    if (tile_rows) n = fill < 16 ? (tile_rows < 16 ? tile_rows : 16) : fill < tile_rows ? fill : tile_rows;
+    const double waves = (double)(((long long)tiles * pair_f + pairs - 1) / pairs);
+    const double walk = waves * (nkb * (.257 + .00045 * n) + (2 * n > G8P_SUM_COLS ? 1.0 : .8));
+    const double t = 5.2 + (walk > memory ? walk : memory);
     if (t < least) least = t, best.n_t = tiles;
   }
   for (int nt = 16; nt <= 128; nt *= 2) {
     if (tile_rows ? nt < tile_rows : nt >= 2 * rows && nt > 16) continue;
-    const long long tiles = (long long)(tile_rows ? n_t : (rows - 1) / nt + 1) * ((N - 1) / G8_BM + 1);
-    for (int splits = 1; splits <= G8_MAX_SPLITS && splits <= nkb && (splits == 1 || tiles * splits <= 2 * sms); ++splits)
-      for (int per_sm = 1; per_sm <= 2; ++per_sm) {
-        const int stages = nt == 16   ? g8_stages<16>(nkb, splits, per_sm)
-                           : nt == 32 ? g8_stages<32>(nkb, splits, per_sm)
-                           : nt == 64 ? g8_stages<64>(nkb, splits, per_sm)
-                                      : g8_stages<128>(nkb, splits, per_sm);
-        if (stages == 0) continue;
-        // Clusters leave SMs over: 132 of 148 are held by blocks in fours, one an SM, 120 in eights.
-        const double held = (double)per_sm * sms * (splits <= 2 ? 1.0 : splits <= 4 ? .89 : .81);
-        const long long blocks = tiles * splits;
-        const double waves = (double)(long long)((blocks + held - 1) / held);
-        const int together = per_sm == 2 && blocks > sms ? 2 : 1;
-        const double shared = together * (16.4 + .128 * nt) / 138, alone = .18 + .0006 * nt;
-        const double walk = waves * ((nkb + splits - 1) / splits) * (shared > alone ? shared : alone);
-        const double t = 3.2 + .004 * nt + (splits > 1 ? .4 + .035 * nt : 0.0) + 2.0 * (waves - 1) + (walk > memory ? walk : memory);
-        if (t < least) least = t, best = {nt, splits, per_sm, 0};
-      }
+    const long long n_f = (N - 1) / G8_BM + 1, tiles = (tile_rows ? live : (rows - 1) / nt + 1) * n_f;
+    const int n = tile_rows && fill < nt ? (fill < 16 ? 16 : fill) : nt;
+    for (int splits = 1; splits <= G8_MAX_SPLITS && splits <= nkb && (splits == 1 || tiles * splits <= 2 * sms); ++splits) {
+      const long long blocks = tiles * splits, grid = tile_rows ? max_tiles * n_f * splits : blocks;
+      int per_sm = g8_per_sm(grid, splits, sms);
+      const auto stages = nt == 16 ? g8_stages<16> : nt == 32 ? g8_stages<32> : nt == 64 ? g8_stages<64> : g8_stages<128>;
+      if (stages(nkb, splits, per_sm) == 0) per_sm = 1;
+      // Clusters leave SMs over: 132 of 148 are held by blocks in fours, one an SM, 120 in eights.
+      const double held = (double)per_sm * sms * (splits <= 2 ? 1.0 : splits <= 4 ? .89 : .81);
+      const double waves = (double)(long long)((blocks + held - 1) / held);
+      const int together = per_sm == 2 && blocks > sms ? 2 : 1;
+      const double shared = together * (16.4 + .128 * n) / 120, alone = .10 + .0006 * n;
+      const double walk = waves * ((nkb + splits - 1) / splits) * (shared > alone ? shared : alone) + 2.7 * (waves - 1);
+      const double stream = memory + .5 * (waves - 1);
+      const double t = 2.1 + .002 * nt + (splits > 1 ? .56 + .027 * n : 0.0) + (walk > stream ? walk : stream) +
+                       .13 * (double)(grid - blocks) / held;
+      if (t < least) least = t, best = {nt, splits, per_sm, 0};
+    }
   }
   return best;
 }
 
-// The same, remembered by the sizes (the estimates of the 60 ways cost part of a microsecond).
-static G8Choice g8_chosen(int rows, int tile_rows, int n_t, int N, int K, long long weight_rows, int sms) {
-  struct Known { int rows, tile_rows, n_t, N, K, sms; long long weight_rows; G8Choice way; };
+// The same, remembered by the sizes (the estimates of the 30 ways cost part of a microsecond).
+static G8Choice g8_chosen(int rows, int tile_rows, int max_tiles, int groups, int N, int K, int sms) {
+  struct Known { int rows, tile_rows, max_tiles, groups, N, K, sms; G8Choice way; };
   static thread_local Known known[64];      // rows 0: empty
-  const unsigned h = (unsigned)rows * 0x9E3779B1u ^ (unsigned)N * 0x85EBCA77u ^ (unsigned)K * 0xC2B2AE3Du ^ (unsigned)n_t * 0x27D4EB2Fu;
+  const unsigned h = (unsigned)rows * 0x9E3779B1u ^ (unsigned)N * 0x85EBCA77u ^ (unsigned)K * 0xC2B2AE3Du ^ (unsigned)max_tiles * 0x27D4EB2Fu;
   Known& k = known[(h ^ h >> 15) % 64];
-  if (k.rows != rows || k.tile_rows != tile_rows || k.n_t != n_t || k.N != N || k.K != K || k.sms != sms || k.weight_rows != weight_rows)
-    k = {rows, tile_rows, n_t, N, K, sms, weight_rows, g8_choose(rows, tile_rows, n_t, N, K, weight_rows, sms)};
+  if (k.rows != rows || k.tile_rows != tile_rows || k.max_tiles != max_tiles || k.groups != groups || k.N != N || k.K != K || k.sms != sms)
+    k = {rows, tile_rows, max_tiles, groups, N, K, sms, g8_choose(rows, tile_rows, max_tiles, groups, N, K, sms)};
   return k.way;
 }
 
@@ -994,7 +1003,7 @@ LLMRS_API int llmrs_gemm_fp8(const void* x, long long x_pitch, const void* xs, l
   const int dev = g8_device(&sms), nkb = (K - 1) / G8_BK + 1;
   int per_sm = 0, n_t = 0;
   if (nt == 0) {
-    const G8Choice way = g8_chosen(x_rows, tile_rows, max_tiles < x_rows ? max_tiles : x_rows, N, K, (long long)groups * N, sms);
+    const G8Choice way = g8_chosen(x_rows, tile_rows, max_tiles, groups, N, K, sms);
     nt = way.nt, splits = way.splits, per_sm = way.per_sm, n_t = way.n_t;
   } else if (splits == 0) {
     splits = 1;
@@ -1017,7 +1026,7 @@ LLMRS_API int llmrs_gemm_fp8(const void* x, long long x_pitch, const void* xs, l
   const long long work = (long long)(grouped ? max_tiles : p.n_t) * p.n_f;
   LLMRS_REQUIRE(work <= 0x7fffffffLL, "%s: too many tiles", what);
   LLMRS_REQUIRE(splits >= 1 && splits <= G8_MAX_SPLITS && splits <= nkb, "%s: 1 to %d parts of k, got %d", what, G8_MAX_SPLITS, splits);
-  if (per_sm == 0) per_sm = work * splits > (splits > 2 ? sms * 4 / 5 : sms) ? 2 : 1;
+  if (per_sm == 0) per_sm = g8_per_sm(work * splits, splits, sms);
   CUtensorMap mw, mx;
   if (const int rc = g8_map(&mw, w, (long long)groups * N, K, w_pitch, G8_BM)) return rc;
   if (const int rc = g8_map(&mx, x, x_rows, K, x_pitch, p.x_box)) return rc;
