@@ -99,7 +99,7 @@ __device__ __forceinline__ void f8_load_pairs(const __nv_bfloat16* p, int left, 
   uint32_t r[9];
 #pragma unroll
   for (int i = 0; i < 9; ++i)
-    r[i] = (FULL || 2 * (32 * i + lane) - odd < left) && (i < 8 || lane < odd) ? __ldg(w + 32 * i + lane) : 0u;
+    r[i] = (FULL || max(2 * (32 * i + lane) - odd, 0) < left) && (i < 8 || lane < odd) ? __ldg(w + 32 * i + lane) : 0u;
   if (odd) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = __funnelshift_r(r[i], __shfl_sync(0xffffffffu, lane == 0 ? r[i + 1] : r[i], lane + 1), 16);
@@ -119,7 +119,7 @@ __device__ __forceinline__ void f8_load_pairs(const float* p, int left, float (&
 #pragma unroll
   for (int i = 0; i < 9; ++i) {
     r[i] = make_float2(0.f, 0.f);
-    if ((FULL || 2 * (32 * i + lane) - odd < left) && (i < 8 || lane < odd)) r[i] = __ldg(w + 32 * i + lane);
+    if ((FULL || max(2 * (32 * i + lane) - odd, 0) < left) && (i < 8 || lane < odd)) r[i] = __ldg(w + 32 * i + lane);
   }
   if (odd) {
 #pragma unroll

@@ -118,6 +118,46 @@ def test_quantize_rows_that_are_picked_and_strided(K, dtype):
             assert not bool(q2[i].view(torch.uint8).any()) and not bool(s2[:, i].view(torch.uint8).any())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_picks_from_no_rows(dtype):
+    """Sources that name nothing, of a matrix without rows that starts in the middle of an aligned pair: zeros, and nothing is read."""
+    from llm_rs_b200 import ops
+    x = _rows(5, 1501, spread=False).to(dtype)
+    src = torch.tensor([0, 4, -1], dtype=torch.int32, device=DEV)
+    for part in (x[3:3], x[5:], x[:0]):
+        q, s = ops.quantize_fp8(part, src)
+        assert not bool(q.view(torch.uint8).any()) and not bool(s.view(torch.uint8).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [511, 512, 514, 516, 528, 1501])
+@pytest.mark.parametrize("off", [0, 1, 2, 4, 7])
+def test_quantize_from_any_address(K, off, dtype):
+    """Rows and pitches of every alignment, with numbers on both sides that must not matter."""
+    from llm_rs_b200 import ops
+    for pitch in (K + off, K + 8 + off):
+        wide = torch.full((6 * pitch + off,), float("inf"), device=DEV, dtype=dtype)
+        x = wide[off:].view(6, pitch)[:, :K]
+        x.copy_(_rows(6, K, seed=K))
+        q, s = ops.quantize_fp8(x)
+        want, e = _exact(x.double())
+        assert bool((q.double() == want).all()) and bool((_scales(s, K)[0] == e).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("inter,block", [(511, 0), (514, 0), (516, 0), (1040, 0), (640, 16), (516, 4), (515, 5), (512, 2), (1040, 80)])
+def test_unit_from_any_address(inter, block, dtype):
+    """Columns of every alignment and order: as the same columns are from dense rows."""
+    from llm_rs_b200 import ops
+    for off in (0, 1, 4, 6):
+        wide = torch.full((5, 2 * inter + off + 3), float("inf"), device=DEV, dtype=dtype)
+        gu = wide[:, off: off + 2 * inter]
+        gu.copy_(_rows(5, 2 * inter, seed=inter, spread=False))
+        both = gu.double().reshape(5, -1, 2, block or inter)
+        gate, up = both[:, :, 0].reshape(5, inter), both[:, :, 1].reshape(5, inter)
+        assert _neighbour(*ops.silu_mul_fp8(gu, block), gate * torch.sigmoid(gate) * up, inter)
+
+
 def _neighbour(q, scales, x, K):
     """Whether (q, scales) stand for a neighbour of the float64 rows x: a whole step of e4m3 (2^-3 of a number in [1, 2)), or of its
     subnormal numbers. A block whose maximum lies at a border may have the scale above it: its step is twice that."""
