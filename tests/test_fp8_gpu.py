@@ -509,3 +509,20 @@ def test_every_way_of_a_product(tokens, features, K, nt, splits):
     ops.check_tc_error(DEV)
     xv, wv = _values(x, xs), _values(w, ws)
     assert bool(((y.double() - xv @ wv.t()).abs() <= _bound(xv, wv, torch.float32, K)).all())
+
+
+@pytest.mark.parametrize("rows,N,K,tile_rows", [(5, 256, 2048, 16), (5, 130, 4096, 32), (300, 512, 1024, 128), (300, 512, 2048, 256)])
+def test_lists_with_room_for_many_more_tiles(rows, N, K, tile_rows):
+    """No tile, one, or a number below zero, of a list with room for fifty: blocks without a tile leave, shared ranges of k or not."""
+    from llm_rs_b200 import ops
+    x, xs = ops.quantize_fp8(_rows(rows, K, seed=1))
+    w, ws = ops.quantize_fp8(_rows(2 * N, K, seed=2))
+    xv, wv = _values(x, xs), _values(w, ws)
+    tiles = torch.tensor([(1, rows - 3, 3)] + [(0, 0, min(rows, tile_rows))] * 49, dtype=torch.int32, device=DEV)
+    for n in (0, 1, -4, 0):
+        out = torch.full((rows, N), 7.0, device=DEV)
+        ops.gemm_fp8_grouped(x, xs, w.unflatten(0, (2, N)), ws, out, tiles, torch.tensor([n], dtype=torch.int32, device=DEV), tile_rows)
+        assert bool((out[: rows - 3 if n == 1 else rows] == 7.0).all())
+        if n == 1:
+            assert bool(((out[-3:].double() - xv[-3:] @ wv[N:].t()).abs() <= _bound(xv[-3:], wv[N:], torch.float32, K)).all())
+    ops.check_tc_error(DEV)
