@@ -304,12 +304,14 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
 
 // ---- the residual sum and the norm ------------------------------------------------------------------------------------
 // h += delta, then h / sqrt(mean(h^2) + eps) * weight in 8 bits; with `rows` row i comes from row rows[i] of h and delta, and h is
-// left as it is. A block per row. The sum of squares is made in float32 by each thread and in double over the threads, and the result
+// left as it is. A block per row. The sum of squares is made in double (in float32 a thread's share of a long row errs by many ulps, all
+// to one side where its numbers are alike, and passes the type's range long before the mean does), and the result
 // is carried in two float32 numbers until it is rounded to float32 once: a number next to a border of e4m3 falls on the formula's side
-// of it but for half an ulp of float32 (4,001 rows of 5,120: 36.8 us; 35.3 with float32 sums and products, 34.9 at 6.45 TB/s).
-__device__ __forceinline__ double f8_block_sum(float own, double2* red) {
+// of it but for half an ulp of float32 (4,001 rows of 5,120: 37.2 us; 36.9
+// with a thread's squares in float32, 34.9 at 6.45 TB/s).
+__device__ __forceinline__ double f8_square(float v, double sum) { return fma((double)v, (double)v, sum); }
+__device__ __forceinline__ double f8_block_sum(double v, double2* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
-  double v = (double)own;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   double* at = reinterpret_cast<double*>(red);
@@ -322,7 +324,7 @@ __device__ __forceinline__ double f8_block_sum(float own, double2* red) {
 }
 
 // 1 / sqrt(mean of the squares + eps) as the sum of two float32 numbers: CUDA's approximate root and one Newton step in double. NaN where
-// the squares pass float32.
+// the mean passes float32.
 struct F8Root { float hi, lo; };
 __device__ __forceinline__ F8Root f8_inverse_root(double squares, double per, float eps) {
   const double mean = squares * per + (double)eps, y = rsqrtf((float)mean);
@@ -374,10 +376,10 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
 #pragma unroll
   for (int i = 0; i < 16; ++i) wt[i] = 0.f;
   f8_load<WAY, false>([&](int c) { return weight + at + c; }, left, wt);
-  float ss = 0.f;
+  double ss[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-  const F8Root inv = f8_inverse_root(f8_block_sum(ss, red), per, eps);
+  for (int i = 0; i < 16; ++i) ss[i % 4] = f8_square(v[i], ss[i % 4]);      // (one chain of sixteen: 37.6 us)
+  const F8Root inv = f8_inverse_root(f8_block_sum(ss[0] + ss[1] + (ss[2] + ss[3]), red), per, eps);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : 32 * i + lane;
@@ -399,7 +401,7 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
   const bool live = from >= 0 && from < h_rows;
   float* hr = h + (live ? (size_t)from * o.width : 0);
   const T* dr = delta && live ? delta + (size_t)from * o.width : nullptr;
-  float ss = 0.f;
+  double ss = 0.0;
   if (live)
     for (int c = threadIdx.x; c < o.width; c += F8_NORM_THREADS) {
       float v = hr[c];
@@ -407,7 +409,7 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
         v += to_float(dr[c]);
         if (!rows) hr[c] = v;
       }
-      ss = fmaf(v, v, ss);
+      ss = f8_square(v, ss);
     }
   const double total = f8_block_sum(ss, red);      // (its barrier also orders the sums above before the loads below)
   const F8Root inv = f8_inverse_root(total, per, eps);

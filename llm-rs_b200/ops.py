@@ -2051,7 +2051,8 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
                     rows: Optional[torch.Tensor] = None):
     """``add_rmsnorm`` with its result in 8 bits: ``h += delta`` (float32 or bfloat16, when given) in place, then ``(q, scales)`` of
     ``h / sqrt(mean(h^2) + eps) * weight``, rounded once. With ``rows`` (int32) only those rows are normed, into row i, and ``h`` is
-    left as it is; an index that names no row gives zeros. A row whose squares pass float32's range becomes NaN."""
+    left as it is; an index that names no row gives zeros. The statistics are made in double; a row whose mean of squares passes
+    float32's range (or holds no number) becomes NaN."""
     for name, t in (("h", h), ("weight", weight)):
         if t.dtype != torch.float32 or not t.is_contiguous():
             raise KernelError(f"{name} must be contiguous float32, got {t.dtype}")
