@@ -307,7 +307,7 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
 // left as it is. A block per row. The sum of squares is made in double (in float32 a thread's share of a long row errs by many ulps, all
 // to one side where its numbers are alike, and passes the type's range long before the mean does), and the result
 // is carried in two float32 numbers until it is rounded to float32 once: a number next to a border of e4m3 falls on the formula's side
-// of it but for half an ulp of float32 (4,001 rows of 5,120: 37.2 us; 36.9
+// of it but for half an ulp of float32 (4,001 rows of 5,120: 37.4 us; 36.9
 // with a thread's squares in float32, 34.9 at 6.45 TB/s).
 __device__ __forceinline__ double f8_square(float v, double sum) { return fma((double)v, (double)v, sum); }
 __device__ __forceinline__ double f8_block_sum(double v, double2* red) {
@@ -323,12 +323,13 @@ __device__ __forceinline__ double f8_block_sum(double v, double2* red) {
   return t;
 }
 
-// 1 / sqrt(mean of the squares + eps) as the sum of two float32 numbers: CUDA's approximate root and one Newton step in double. NaN where
-// the mean passes float32.
+// 1 / sqrt(mean) as the sum of two float32 numbers: CUDA's approximate root and one Newton step in double (its root in double took 38.5
+// us). NaN where the mean of the squares, with the eps, passes float32. Without an eps a small row's mean may lie below float32: the
+// row is then normed 2^100 times as large (a branch that a row takes as a whole; always multiplying took 38.1 us).
+constexpr float F8_SMALL = 0x1p-100f, F8_UP = 0x1p100f;
 struct F8Root { float hi, lo; };
-__device__ __forceinline__ F8Root f8_inverse_root(double squares, double per, float eps) {
-  const double mean = squares * per + (double)eps, y = rsqrtf((float)mean);
-  const double root = y > 0.0 ? y * (1.5 - 0.5 * mean * y * y) : (double)NAN;
+__device__ __forceinline__ F8Root f8_inverse_root(double mean) {
+  const double y = rsqrtf((float)mean), root = y > 0.0 ? y * (1.5 - 0.5 * mean * y * y) : (double)NAN;
   F8Root r;
   r.hi = (float)root, r.lo = (float)(root - (double)r.hi);
   return r;
@@ -379,7 +380,13 @@ f8_norm_kernel(float* __restrict__ h, const T* __restrict__ delta, const float* 
   double ss[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
   for (int i = 0; i < 16; ++i) ss[i % 4] = f8_square(v[i], ss[i % 4]);      // (one chain of sixteen: 37.6 us)
-  const F8Root inv = f8_inverse_root(f8_block_sum(ss[0] + ss[1] + (ss[2] + ss[3]), red), per, eps);
+  double mean = f8_block_sum(ss[0] + ss[1] + (ss[2] + ss[3]), red) * per + (double)eps;
+  if ((float)mean < F8_SMALL) {
+    mean *= (double)F8_UP * (double)F8_UP;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= F8_UP;
+  }
+  const F8Root inv = f8_inverse_root(mean);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : 32 * i + lane;
@@ -411,8 +418,10 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
       }
       ss = f8_square(v, ss);
     }
-  const double total = f8_block_sum(ss, red);      // (its barrier also orders the sums above before the loads below)
-  const F8Root inv = f8_inverse_root(total, per, eps);
+  double mean = f8_block_sum(ss, red) * per + (double)eps;      // (its barrier also orders the sums above before the loads below)
+  const float up = (float)mean < F8_SMALL ? F8_UP : 1.0f;
+  mean *= (double)up * (double)up;
+  const F8Root inv = f8_inverse_root(mean);
   for (int word = warp; word < o.n_words; word += F8_NORM_THREADS / 32) {
     const int at = word * F8_WORD, left = o.width - at;
     float v[16];
@@ -423,7 +432,7 @@ f8_norm_long_kernel(float* __restrict__ h, const T* __restrict__ delta, const fl
       if (live && c < o.width) {
         v[i] = hr[c];
         if (dr && rows) v[i] += to_float(dr[c]);
-        v[i] = f8_scaled(v[i], inv, weight[c]);
+        v[i] = f8_scaled(v[i] * up, inv, weight[c]);
       }
     }
     f8_store<F8_ONES, false>(v, o.q + (size_t)r * o.pitch + at, left, o.words + (size_t)word * o.rows + r);

@@ -78,6 +78,19 @@ def test_norm_of_large_rows(K):
         assert _nearest(q, s, _norm(h.double(), w.double(), eps), NORM_SLACK)
 
 
+@pytest.mark.parametrize("K", [512, 515, 4096, 17000])
+@pytest.mark.parametrize("eps", [0.0, 1e-6, 1e-42])
+def test_norm_of_small_rows(K, eps):
+    """Squares, and their mean, below what float32 holds; without an eps such rows are normed as any others, and empty rows are 0 / 0."""
+    from llm_rs_b200 import ops
+    w = 1 + 0.1 * _rows(1, K, seed=1, spread=False)[0]
+    h = _rows(6, K, seed=2, spread=False) * torch.tensor([1e-15, 1e-19, 1e-22, 1e-25, 1e-31, 1e-36], device=DEV)[:, None]
+    q, s = ops.add_rmsnorm_fp8(h, None, w, eps)
+    assert _nearest(q, s, _norm(h.double(), w.double(), eps), NORM_SLACK)
+    q, s = ops.add_rmsnorm_fp8(torch.zeros((2, K), device=DEV), None, w, eps)
+    assert bool(q.float().isnan().all()) if eps == 0 else not bool(q.view(torch.uint8).any())
+
+
 @pytest.mark.parametrize("K", [512, 515, 17000])
 def test_norm_of_rows_whose_mean_passes_float32(K):
     """The mean of the squares is what decides, not how they are dealt to threads: just below the largest float32 a row is normed, just
