@@ -1,4 +1,4 @@
-"""Rows in 8 bits that are computed on the way, held to the nearest number.
+"""Rows in 8 bits that are computed on the way (the norm, the gated unit), held to the nearest number.
 
 What a kernel computes before its one rounding to e4m3 errs by a share `slack` of itself, which follows from its operations. So the
 quantised number errs from the exact one by half a step of e4m3 (2^-4 of the number's power of two, 2^-10 * 2^E where it is subnormal)
@@ -11,6 +11,7 @@ from test_fp8_gpu import _exact, _rows, _scales, _values
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+INF, NAN = float("inf"), float("nan")
 
 
 def _nearest(q, scales, x, slack):
@@ -105,3 +106,51 @@ def test_norm_of_rows_whose_mean_passes_float32(K):
     good = h[0::2]
     assert _nearest(q[0::2], s[:, 0::2], _norm(good.double(), w.double()), NORM_SLACK)
     assert bool(q[1].float().isnan().all())
+
+
+# -- the gated unit ---------------------------------------------------------------------------------------------------
+def _unit(gate, up, unit=(INF, 1.0, 0.0)):
+    limit, alpha, shift = unit
+    g, u = gate.clamp(max=limit), up.clamp(-limit, limit)
+    t = alpha * g
+    a = torch.exp(-t.abs() / 2)                       # exp(t) = a * a for t < 0: no factor leaves float64
+    return torch.where(t < 0, g * a / (1 + a * a) * (u + shift) * a, g / (1 + a * a) * (u + shift)), t
+
+
+def _unit_slack(t):
+    # Approximate power (2^-22.5 of itself; its square where the gate is far below zero: twice that), reciprocal (2^-23) and up to five
+    # roundings of 2^-24; the power's argument errs by three roundings of itself: |t| 3 * 2^-24 of the power.
+    return 2.0 ** -19.5 + 3 * t.abs() * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,inter,block", [(3, 640, 64), (33, 12288, 64), (2, 333, 0), (7, 520, 8), (5, 515, 5), (600, 1000, 0)])
+def test_unit_is_the_nearest_number(rows, inter, block, dtype):
+    from llm_rs_b200 import ops
+    gu = (2 * _rows(rows, 2 * inter, seed=inter, spread=False)).to(dtype)
+    both = gu.double().reshape(rows, -1, 2, block or inter)
+    gate, up = both[:, :, 0].reshape(rows, inter), both[:, :, 1].reshape(rows, inter)
+    for unit in ((INF, 1.0, 0.0), (1.5, 1.702, 1.0)):
+        x, t = _unit(gate, up, unit)
+        assert _nearest(*ops.silu_mul_fp8(gu, block, unit=unit), x, _unit_slack(t))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("inter", [512, 516, 515])
+@pytest.mark.parametrize("unit", [(INF, 1.0, 0.0), (7.0, 1.702, 1.0), (INF, 1.702, 0.0)])
+def test_unit_of_what_is_no_number(unit, inter, dtype):
+    """A NaN in the gate or the up becomes a NaN, whatever the unit's limit is; an infinity that no limit holds does too. Their neighbours
+    are as without them."""
+    from llm_rs_b200 import ops
+    gu = _rows(4, 2 * inter, seed=inter, spread=False).to(dtype)
+    gu[:, 5], gu[:, 200], gu[:, inter + 300] = 4.0, 4.0, 4.0      # (their blocks' largest results are elsewhere)
+    gu[:, [100, 130, 300, 350, 400]], gu[:, [inter + c for c in (100, 130, 300, 350, 400)]] = 5.0, 5.0
+    clean, _ = ops.silu_mul_fp8(gu, unit=unit)
+    gu[0, 5], gu[1, inter + 300], gu[2, 200], gu[3, inter + 300] = NAN, NAN, INF, -INF
+    q, _ = ops.silu_mul_fp8(gu, unit=unit)
+    bad = torch.zeros((4, inter), dtype=torch.bool, device=DEV)
+    bad[0, 5] = bad[1, 300] = True
+    if unit[0] == INF:
+        bad[2, 200] = bad[3, 300] = True
+    assert bool(q.float()[bad].isnan().all()) and bool(q.float()[~bad].isfinite().all())
+    assert bool((q.float() == clean.float())[0][~bad[0]].all()) and bool((q.float() == clean.float())[1][~bad[1]].all())
