@@ -2034,7 +2034,7 @@ def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
 def silu_mul_fp8(gate_up: torch.Tensor, block: int = 0, unit=PLAIN_SILU):
     """``silu_mul`` with its result in 8 bits: ``(q, scales)`` of ``silu(gate) * up`` for ``gate_up`` [rows, 2I] that holds gate and
     up in alternating runs of ``block`` columns (0: I gate columns, then I up columns; else a divisor of I). The unit is
-    computed in float32 and rounded once."""
+    computed in float32, with an error of some 2^-21 of itself (and 2^-23 |alpha gate|), and rounded once."""
     rows, two, stride, code = _fp8_rows(gate_up, "gate_up")
     inter = two // 2
     if two % 2 or block < 0 or (block and inter % block):

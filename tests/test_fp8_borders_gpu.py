@@ -136,6 +136,25 @@ def test_unit_is_the_nearest_number(rows, inter, block, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("inter,block", [(512, 64), (516, 0), (515, 0), (515, 5), (1040, 16)])
+@pytest.mark.parametrize("low,high", [(-87.0, -84.0), (-92.0, -86.0), (-130.0, -88.0), (-170.0, -100.0), (-95.0, 3.0)])
+def test_unit_of_gates_far_below_zero(low, high, inter, block, dtype):
+    """Blocks whose gates all are far below zero, beside ups that bring the result back into range: e^gate is below what float32 holds."""
+    from llm_rs_b200 import ops
+    g = torch.Generator(device=DEV)
+    g.manual_seed(int(-low) + inter)
+    gate = torch.rand((5, inter), generator=g, device=DEV) * (high - low) + low
+    up = torch.randn((5, inter), generator=g, device=DEV) * 1e30
+    b = block or inter
+    gu = torch.stack([gate.reshape(5, -1, b), up.reshape(5, -1, b)], dim=2).reshape(5, 2 * inter).to(dtype)
+    both = gu.double().reshape(5, -1, 2, b)
+    gate, up = both[:, :, 0].reshape(5, inter), both[:, :, 1].reshape(5, inter)
+    for unit in ((INF, 1.0, 0.0), (1e38, 1.0, 0.0), (1e38, 1.25, 0.0)):
+        x, t = _unit(gate, up, unit)
+        assert _nearest(*ops.silu_mul_fp8(gu, block, unit=unit), x, _unit_slack(t))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("inter", [512, 516, 515])
 @pytest.mark.parametrize("unit", [(INF, 1.0, 0.0), (7.0, 1.702, 1.0), (INF, 1.702, 0.0)])
 def test_unit_of_what_is_no_number(unit, inter, dtype):
