@@ -30,9 +30,6 @@ class EngineConfig:
     page_size: int = 16                  # llm-core/src/backends/candle.rs:827
     dtype: str = "bfloat16"              # "bfloat16" or "float32"
     device: str = "cuda:0"
-    # "stored", or "fp8": attention projections, feed-forwards and experts in 8 bits (bfloat16 engines; the weights are
-    # quantised as they are loaded, the activations in every step).
-    products: str = "stored"
     max_requests: int = 64               # live requests (state slots)
     max_tokens_per_step: int = 2048
     prefill_chunk: int = 512
@@ -40,6 +37,9 @@ class EngineConfig:
     # Queue the next step on the GPU before the last one's tokens are read back (they feed
     # the next step on the device); ``step()`` then reports a step's tokens one call later.
     async_steps: bool = True
+    # "stored", or "fp8": attention projections, feed-forwards and experts in 8 bits (bfloat16 engines; the weights are
+    # quantised as they are loaded, the activations in every step).
+    products: str = "stored"
 
 
 class Engine:
