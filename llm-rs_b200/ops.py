@@ -1933,6 +1933,11 @@ def rglru_step(u: torch.Tensor, w: torch.Tensor, r_bias: torch.Tensor, i_bias: t
 # the least integer >= -127 with which the block's largest magnitude is at most 448. Places past a row's last block hold 2^-127.
 FP8, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 FP8_BLOCK = 128         # numbers of a row that share a scale
+FP8_MOST = 0x7ffffe00   # rows, or numbers of a row, at most: the kernels count both in 32 bits, and the arguments are cut to them
+
+
+def _fp8_too_many(name: str, *sizes: int) -> None:
+    raise KernelError(f"{name}: at most {FP8_MOST} rows, and numbers of a row, got {sizes}")
 
 
 _fp8_entries = {}
@@ -1981,6 +1986,8 @@ def _fp8_rows(x: torch.Tensor, name: str):
     if x.dim() != 2 or x.size(1) < 1:
         raise KernelError(f"{name} must be [rows, numbers], got {tuple(x.shape)}")
     rows, K = x.shape
+    if rows > FP8_MOST or K > FP8_MOST:
+        _fp8_too_many(name, rows, K)
     stride, one = x.stride()
     if one != 1 and K > 1:
         raise KernelError(f"{name} must have dense rows, got sizes {tuple(x.shape)} strides {x.stride()}")
@@ -1994,6 +2001,8 @@ def _fp8_operand(q: torch.Tensor, scales: torch.Tensor, name: str):
     if q.dim() != 2 or q.size(1) < 1:
         raise KernelError(f"{name} must be [rows, K], got {tuple(q.shape)}")
     rows, K = q.shape
+    if rows > FP8_MOST or K > FP8_MOST:
+        _fp8_too_many(name, rows, K)
     words = (K + 511) >> 9
     if scales.shape != (words, rows, 4):
         raise KernelError(f"{name} is {tuple(q.shape)}: its scales must be {(words, rows, 4)}, got {tuple(scales.shape)}")
@@ -2022,8 +2031,10 @@ def quantize_fp8(x: torch.Tensor, src: Optional[torch.Tensor] = None):
     if src is not None:
         if src.dtype != torch.int32 or src.dim() != 1 or not src.is_contiguous():
             raise KernelError(f"src must be a contiguous int32 vector, got {src.dtype} {tuple(src.shape)}")
-    stream = _fp8_stream(x, src)
     n = rows if src is None else src.numel()
+    if n > FP8_MOST:
+        _fp8_too_many("src", n)
+    stream = _fp8_stream(x, src)
     q, scales, pitch = _fp8_new(x, n, K)
     fn = _fp8_entries.get("llmrs_quantize_fp8") or _fp8_entry("llmrs_quantize_fp8", 11, wide=(0, 2, 4, 5, 6, 7, 10))
     _check(fn(x.data_ptr(), code, stride, rows, None if src is None else src.data_ptr(), q.data_ptr(), pitch,
@@ -2063,8 +2074,10 @@ def add_rmsnorm_fp8(h: torch.Tensor, delta: Optional[torch.Tensor], weight: torc
         raise KernelError(f"delta {tuple(delta.shape)} ({delta.dtype}) must be float32 or bfloat16 rows like h {tuple(h.shape)}")
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
         raise KernelError(f"rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
-    stream = _fp8_stream(h, delta, weight, rows)
     m = n if rows is None else rows.numel()
+    if m > FP8_MOST:
+        _fp8_too_many("rows", m)
+    stream = _fp8_stream(h, delta, weight, rows)
     q, scales, pitch = _fp8_new(h, m, K)
     fn = _fp8_entries.get("llmrs_add_rmsnorm_fp8") or _fp8_entry("llmrs_add_rmsnorm_fp8", 13, (6,), (0, 1, 3, 4, 7, 8, 9, 12))
     _check(fn(h.data_ptr(), None if delta is None else delta.data_ptr(), F32 if delta is None else _DTYPE_CODE[delta.dtype],
@@ -2140,6 +2153,8 @@ def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
         raise KernelError(f"tiles of 1 to 256 rows, got {tile_rows}")
     if tiles.dtype != torch.int32 or tiles.dim() != 2 or tiles.size(1) != 3 or not tiles.is_contiguous():
         raise KernelError(f"tiles must be contiguous int32 [tiles, 3], got {tiles.dtype} {tuple(tiles.shape)}")
+    if tiles.size(0) > FP8_MOST:
+        _fp8_too_many("tiles", tiles.size(0))
     if n_tiles.dtype != torch.int32 or n_tiles.numel() != 1:
         raise KernelError(f"n_tiles must be one int32, got {n_tiles.dtype} {tuple(n_tiles.shape)}")
     stream = _fp8_stream(x, x_scales, w, w_scales, out, tiles, n_tiles)

@@ -11,3 +11,34 @@ def test_engine_fields_keep_their_places():
     c = EngineConfig("folder", 1024, 16, "bfloat16", "cuda:0", 7, 300, 200, False, False)
     assert (c.max_requests, c.max_tokens_per_step, c.prefill_chunk, c.cuda_graphs, c.async_steps, c.products) == (7, 300, 200, False, False, "stored")
     assert EngineConfig("folder", products="fp8").products == "fp8"
+
+
+def _meta(*shape, dtype):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("many", [0x7ffffe01, 2 ** 31, 2 ** 32, 2 ** 32 + 8])
+def test_sizes_past_32_bits_are_refused(many):
+    """They would reach the kernels cut to 32 bits: 2^32 rows as none, 2^32 + 8 as eight."""
+    E4, E8, I32 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.int32
+
+    def refused(f, *a, **k):
+        with pytest.raises(ops.KernelError, match="at most 2147483136 rows"):
+            f(*a, **k)
+    narrow, wide, index = _meta(many, 2, dtype=torch.bfloat16), _meta(2, many, dtype=torch.bfloat16), _meta(many, dtype=I32)
+    for x in (narrow, wide):
+        refused(ops.quantize_fp8, x)
+        refused(ops.silu_mul_fp8, x)
+        refused(ops.add_rmsnorm_fp8, x.float(), None, _meta(x.size(1), dtype=torch.float32), 1e-6)
+    refused(ops.quantize_fp8, _meta(4, 64, dtype=torch.float32), index)
+    refused(ops.add_rmsnorm_fp8, _meta(4, 64, dtype=torch.float32), None, _meta(64, dtype=torch.float32), 1e-6, rows=index)
+    few = (_meta(4, 16, dtype=E4), _meta(1, 4, 4, dtype=E8))
+    tall, long = (_meta(many, 16, dtype=E4), _meta(1, many, 4, dtype=E8)), (_meta(4, many, dtype=E4), _meta((many + 511) // 512, 4, 4, dtype=E8))
+    for x, w in ((tall, few), (few, tall), (long, long)):
+        refused(ops.gemm_fp8, *x, *w)
+    tiles, n = _meta(3, 3, dtype=I32), _meta(1, dtype=I32)
+    grouped = lambda x, w, g, tiles: ops.gemm_fp8_grouped(*x, w[0].unflatten(0, (g, -1)), w[1], _meta(x[0].size(0), w[0].size(0) // g,
+                                                          dtype=torch.float32), tiles, n, 64)
+    refused(grouped, tall, few, 2, tiles)
+    refused(grouped, few, tall, many, tiles)
+    refused(grouped, few, few, 2, _meta(many, 3, dtype=I32))
