@@ -210,12 +210,37 @@ def _cost_fp8(x, x_scales, w, w_scales, out=None, epilogue="store", out_dtype=to
 
 
 def _cost_fp8_grouped(x, x_scales, w, w_scales, out, *a, **k):
-    return _cost_grouped(x, w, out, None, None, None)
+    label, nbytes, flops = _cost_grouped(x, w, out, None, None, None)
+    scales = w_scales.size(0) * 4                      # of a row, for every 512 numbers a word of four
+    G, N = w.size(0), w.size(1)
+    touched = G * (1.0 - (1.0 - 1.0 / G) ** max(out.size(0), 1))
+    return label, nbytes + int(touched * N * scales) + _nbytes(x_scales), flops
+
+
+def _rows8_bytes(rows: int, K: int) -> int:
+    return rows * (K + -(-K // 512) * 4)
+
+
+def _cost_quantize_fp8(x, src=None):
+    rows, K = x.size(0) if src is None else src.numel(), x.size(1)
+    # (With sources every row of x that one of them names is read once, at most as many as there are.)
+    return f"{rows}x{K}", min(rows, x.size(0)) * K * x.element_size() + _nbytes(src) + _rows8_bytes(rows, K), 0.0
+
+
+def _cost_unit_fp8(gate_up, block=0, unit=None):
+    rows, K = gate_up.size(0), gate_up.size(1) // 2
+    return f"{rows}x{K}", _nbytes(gate_up) + _rows8_bytes(rows, K), 0.0
+
+
+def _cost_norm_fp8(h, delta, weight, eps, rows=None):
+    n, K = h.size(0) if rows is None else rows.numel(), h.size(1)
+    per_number = 4 + (0 if delta is None else delta.element_size() + (4 if rows is None else 0))      # the sum goes back into h
+    return f"{n}x{K}", min(n, h.size(0)) * K * per_number + _nbytes(weight, rows) + _rows8_bytes(n, K), 0.0
 
 
 WRAPPED: Dict[str, Callable] = {
-    "gemm_fp8": _cost_fp8, "gemm_fp8_grouped": _cost_fp8_grouped, "quantize_fp8": _cost_rows(0), "silu_mul_fp8": _cost_rows(0),
-    "add_rmsnorm_fp8": _cost_rows(0),
+    "gemm_fp8": _cost_fp8, "gemm_fp8_grouped": _cost_fp8_grouped, "quantize_fp8": _cost_quantize_fp8, "silu_mul_fp8": _cost_unit_fp8,
+    "add_rmsnorm_fp8": _cost_norm_fp8,
     "add_two_rmsnorm": _cost_two_norms, "rglru_gates": _cost_gates, "rglru_step": _cost_rglru_step,
     "rglru_scan": lambda ab, y, y_bias, state, ctx: (f"{ab.size(0)} tokens", _nbytes(ab) + ab.size(0) * ab.size(1) * 2 * y.element_size()
                                                      + 2 * ctx.n_requests * ab.size(1) * 4, 0.0),

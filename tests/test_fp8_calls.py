@@ -42,3 +42,28 @@ def test_sizes_past_32_bits_are_refused(many):
     refused(grouped, tall, few, 2, tiles)
     refused(grouped, few, tall, many, tiles)
     refused(grouped, few, few, 2, _meta(many, 3, dtype=I32))
+
+
+def test_bytes_that_the_profiler_counts():
+    """What each operator has to read and to write, whatever it is called with."""
+    from llm_rs_b200.profiling import WRAPPED
+    E4, E8, I32, BF, F32 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.int32, torch.bfloat16, torch.float32
+    cost = lambda name, *a, **k: WRAPPED[name](*a, **k)[1]
+    eight = lambda rows, K: rows * K + rows * ((K + 511) // 512) * 4
+    x, src = _meta(10, 1000, dtype=BF), _meta(35, dtype=I32)
+    assert cost("quantize_fp8", x) == 10 * 1000 * 2 + eight(10, 1000)
+    assert cost("quantize_fp8", x.float()) == 10 * 1000 * 4 + eight(10, 1000)
+    assert cost("quantize_fp8", x, src) == 10 * 1000 * 2 + 35 * 4 + eight(35, 1000)
+    assert cost("quantize_fp8", x, src[:3]) == 3 * 1000 * 2 + 3 * 4 + eight(3, 1000)
+    assert cost("silu_mul_fp8", x, block=100, unit=(7.0, 1.0, 0.0)) == 10 * 1000 * 2 + eight(10, 500)
+    h, w = _meta(10, 1000, dtype=F32), _meta(1000, dtype=F32)
+    assert cost("add_rmsnorm_fp8", h, None, w, 1e-6) == 10 * 1000 * 4 + 4000 + eight(10, 1000)
+    assert cost("add_rmsnorm_fp8", h, x, w, 1e-6) == 10 * 1000 * (4 + 2 + 4) + 4000 + eight(10, 1000)
+    assert cost("add_rmsnorm_fp8", h, x, w, 1e-6, rows=src[:4]) == 4 * 1000 * (4 + 2) + 4 * 4 + 4000 + eight(4, 1000)
+    q, s = _meta(10, 1000, dtype=E4), _meta(2, 10, 4, dtype=E8)
+    v, t = _meta(300, 1000, dtype=E4), _meta(2, 300, 4, dtype=E8)
+    assert cost("gemm_fp8", q, s, v, t) == eight(10, 1000) + eight(300, 1000) + 10 * 300 * 2
+    assert cost("gemm_fp8", q, s, v, t, out=_meta(10, 300, dtype=F32), epilogue="residual") == eight(10, 1000) + eight(300, 1000) + 10 * 300 * 8
+    # Three groups and ten rows dealt evenly: 3 (1 - (2/3)^10) groups have one.
+    got = cost("gemm_fp8_grouped", q, s, v.unflatten(0, (3, 100)), t, _meta(10, 100, dtype=BF), _meta(5, 3, dtype=I32), _meta(1, dtype=I32), 64)
+    assert abs(got - (3 * (1 - (2 / 3) ** 10) * eight(100, 1000) + eight(10, 1000) + 10 * 100 * 2)) <= 2
