@@ -272,6 +272,10 @@ WRAPPED: Dict[str, Callable] = {
 }
 
 
+# Tensor rate of an entry point as a multiple of the bfloat16 rate that a report is made against.
+RATES: Dict[str, float] = {"gemm_fp8": 2.0, "gemm_fp8_grouped": 2.0}
+
+
 def device_peaks() -> Tuple[float, float]:
     """(GB/s, TFLOP/s) to report against: what a file MEASURED_PEAKS.json in the working directory or beside the
     package says (keys hbm_gbs, bf16_tflops), else the nominal figures of a B200 (7,700 GB/s, 2,250 TFLOP/s)."""
@@ -343,7 +347,7 @@ class Profiler:
         rows = []
         for cls, (n, us, nbytes, flops) in agg.items():
             gbs, tf = nbytes / us / 1e3, flops / us / 1e6
-            f_mem, f_math = gbs / self.hbm_gbs, tf / self.tflops
+            f_mem, f_math = gbs / self.hbm_gbs, tf / (self.tflops * RATES.get(cls.split("[")[0], 1.0))
             rows.append({"class": cls, "calls": n, "us_total": round(us, 1), "us_each": round(us / n, 2),
                          "share": round(us / total, 4), "bytes_each": int(nbytes / n), "flops_each": flops / n,
                          "gb_s": round(gbs, 1), "tflop_s": round(tf, 2), "bound": "hbm" if f_mem >= f_math else "tensor",

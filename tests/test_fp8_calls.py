@@ -67,3 +67,21 @@ def test_bytes_that_the_profiler_counts():
     # Three groups and ten rows dealt evenly: 3 (1 - (2/3)^10) groups have one.
     got = cost("gemm_fp8_grouped", q, s, v.unflatten(0, (3, 100)), t, _meta(10, 100, dtype=BF), _meta(5, 3, dtype=I32), _meta(1, dtype=I32), 64)
     assert abs(got - (3 * (1 - (2 / 3) ** 10) * eight(100, 1000) + eight(10, 1000) + 10 * 100 * 2)) <= 2
+
+
+def test_products_in_8_bits_are_reported_against_their_own_rate(monkeypatch):
+    from llm_rs_b200.profiling import Profiler
+
+    class Event:
+        def __init__(self, ms):
+            self.ms = ms
+
+        def elapsed_time(self, other):
+            return other.ms - self.ms
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    p = Profiler(hbm_gbs=1000.0, tflops=1.0)
+    # A millisecond each: 1e9 operations are the bfloat16 rate, half of the 8-bit rate; 3e8 bytes are 0.3 of the memory's.
+    for name in ("gemm_bf16[8x8]", "gemm_fp8[8x8]", "gemm_fp8_grouped[2x8x8]"):
+        p._calls.append((name, 3e8, 1e9, Event(0.0), Event(1.0)))
+    got = {r["class"].split("[")[0]: (r["frac"], r["bound"]) for r in p.classes()}
+    assert got == {"gemm_bf16": (1.0, "tensor"), "gemm_fp8": (0.5, "tensor"), "gemm_fp8_grouped": (0.5, "tensor")}
