@@ -106,11 +106,8 @@ __device__ __forceinline__ bool g8_all_of_four(bool ok) {
 __device__ __forceinline__ void g8_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void g8_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // (In line throughout: a call would make a role's registers spill.)
-__device__ __forceinline__ bool g8_wait_slow(uint32_t bar, uint32_t parity, uint32_t limit, volatile int* abort_flag) {
-  return mbar_wait(bar, parity, limit, abort_flag);
-}
 __device__ __forceinline__ bool g8_wait(uint32_t bar, uint32_t parity, uint32_t limit, volatile int* abort_flag) {
-  return mbar_try_wait(bar, parity) || g8_wait_slow(bar, parity, limit, abort_flag);
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, limit, abort_flag);
 }
 __device__ __forceinline__ void g8_prefetch(const CUtensorMap* map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
@@ -553,7 +550,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 constexpr int G8P_THREADS = 448, G8P_EPI_WARP = 6, G8P_STAGES = 6, G8P_NT = 256;
 constexpr uint32_t G8P_STAGE_BYTES = G8_A_BYTES + G8P_NT / 2 * G8_BK;
 constexpr int G8P_SLOT_COLS = 12, G8P_SUM_COLS = 512 - G8_SLOTS * G8P_SLOT_COLS, G8P_BARS = 2 * G8P_STAGES + 2 * G8_SLOTS + 5;
-constexpr size_t G8P_SMEM = 1024 + (size_t)G8P_STAGES * G8P_STAGE_BYTES + G8P_BARS * 8 + 16;
+constexpr size_t G8P_SMEM = 1024 + (size_t)G8P_STAGES * G8P_STAGE_BYTES + G8P_BARS * 8 + 16;      // (four words behind the barriers)
 
 // A copy into this block's shared memory whose bytes are counted by a barrier that may lie in the pair's other block.
 __device__ __forceinline__ void g8_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c0, int c1) {
@@ -619,6 +616,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   uint64_t* bars = reinterpret_cast<uint64_t*>(stages + (size_t)G8P_STAGES * G8P_STAGE_BYTES);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + G8P_BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* theirs = abort_flag + 1;      // copies that the other block had requested when it gave up; -1: it did not
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t full0 = tc_smem(bars), empty0 = full0 + 8 * G8P_STAGES, sc_full0 = empty0 + 8 * G8P_STAGES,
                  sc_empty0 = sc_full0 + 8 * G8_SLOTS, acc_full = sc_empty0 + 8 * G8_SLOTS, acc_empty = acc_full + 16,
@@ -636,6 +634,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       g8_prefetch_map(&map_w);
       g8_prefetch_map(&map_x);
       *abort_flag = 0;
+      *theirs = -1;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -802,23 +801,39 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    // The block gave up. The MMAs that were issued must be done before tensor memory is freed, and the copies that were requested
-    // must have landed (the leader's barriers count both blocks' bytes; the peer stays until the cluster barrier below).
+    // The block gave up. The MMAs that were issued must be done before tensor memory is freed.
     if (rank == 0 && warp == 1) {
       if (tc_elect_one()) g8_commit_pair_local(drain_bar);
       __syncwarp();
       mbar_drain(drain_bar, 0, p.wait_limit);
-    } else if (rank == 0 && tid == 0) {
-      for (int i = copies > G8P_STAGES ? copies - G8P_STAGES : 0; i < copies; ++i)
-        if (i != p.test_skip_kb) mbar_drain(full0 + 8 * (i % G8P_STAGES), (uint32_t)(i / G8P_STAGES) & 1, p.wait_limit);
+    } else if (tid == 0) {
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(g8_map_rank(tc_smem(const_cast<int*>(theirs)), rank ^ 1)), "r"(copies) : "memory");
+      if (p.error_flag) atomicExch(p.error_flag, 1);
     }
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 1);
     __syncthreads();
   }
   // Neither block may free tensor memory or leave while the other still computes into it or signals its barriers.
   tc_fence_before();
   g8_cluster_arrive();
   g8_cluster_wait();
+  if (*abort_flag || *theirs >= 0) {      // (the same in both blocks)
+    // The copies that were requested must have landed in both. The leader's barriers count them: of a stage that only the other
+    // block came to (it gave up later) the leader has still to say how many bytes are on their way.
+    if (rank == 0 && tid == 0) {
+      for (int i = copies > G8P_STAGES ? copies - G8P_STAGES : 0; i < max(copies, *theirs); ++i) {
+        const uint32_t bar = full0 + 8 * (i % G8P_STAGES);
+        if (i == p.test_skip_kb) continue;
+        if (i >= copies) {
+          const int half = g8_pair_n(g8_tile(p, pair + i / nkb * n_pairs, n_row_tiles, 2 * G8_BM).rows) / 2;
+          mbar_expect_tx(bar, G8_A_BYTES + (uint32_t)((half + p.x_box - 1) / p.x_box * p.x_box) * G8_BK);
+        }
+        mbar_drain(bar, (uint32_t)(i / G8P_STAGES) & 1, p.wait_limit);
+      }
+    }
+    __syncthreads();
+    g8_cluster_arrive();
+    g8_cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
