@@ -1951,7 +1951,20 @@ def _fp8_entry(name: str, n_args: int, floats=(), wide=()):
         fn = getattr(_lib(), name)
         fn.argtypes = [ctypes.c_float if i in floats else ctypes.c_void_p if i in wide else ctypes.c_int for i in range(n_args)]
         _fp8_entries[name] = fn
+        if not torch.cuda.is_current_stream_capturing():      # (operands are made before a product is captured)
+            tc_error_flag(torch.device("cuda", torch.cuda.current_device()))
     return fn
+
+
+def _fp8_flag(device: torch.device) -> int:
+    """The address of the word in which the products report a wait that ran out. One made while a graph is captured would be the
+    graph's own: its replays would empty it."""
+    flag = _tc_flags.get(device)
+    if flag is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError("the first call on a device must not be captured: quantise the operands, or run one product, before")
+        flag = tc_error_flag(device)
+    return flag.data_ptr()
 
 
 def _fp8_new(like: torch.Tensor, rows: int, K: int):
@@ -2118,7 +2131,7 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
         stream = _fp8_stream(x, x_scales, w, w_scales, out)
     _check((_fp8_entries.get("llmrs_gemm_fp8") or _fp8_product())(
         x_at, x_pitch, xs_at, xs, tokens, w_at, w_pitch, ws_at, ws, out.data_ptr(), ldo, code, add, features, K, 1, None, None, 0, 0,
-        0, 0, tc_error_flag(x.device).data_ptr(), stream), "gemm_fp8")
+        0, 0, _fp8_flag(x.device), stream), "gemm_fp8")
     return out
 
 
@@ -2160,6 +2173,6 @@ def gemm_fp8_grouped(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w
     stream = _fp8_stream(x, x_scales, w, w_scales, out, tiles, n_tiles)
     _check((_fp8_entries.get("llmrs_gemm_fp8") or _fp8_product())(
         x_at, x_pitch, xs_at, xs, rows, w_at, w_pitch, ws_at, ws, out.data_ptr(), out.stride(0), _DTYPE_CODE[out.dtype], 0, N, K, G,
-        tiles.data_ptr(), n_tiles.data_ptr(), tiles.size(0), tile_rows, 0, 0, tc_error_flag(x.device).data_ptr(), stream),
+        tiles.data_ptr(), n_tiles.data_ptr(), tiles.size(0), tile_rows, 0, 0, _fp8_flag(x.device), stream),
         "gemm_fp8_grouped")
     return out

@@ -131,3 +131,40 @@ def test_pairs_and_few_tokens_on_two_streams_at_once():
     for ys, y in zip(got, alone):
         assert all(bool((z == y).all()) for z in ys)
     ops.check_tc_error(DEV)
+
+
+def test_a_first_product_that_is_captured_reports_too():
+    """Operands made, then the process's first product captured: the word that a wait which runs out is reported in is not the
+    graph's own, to be emptied by its replays. Without any call before it, the product is refused."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from llm_rs_b200 import ops
+a, b = (torch.zeros((n, 256), dtype=torch.float8_e4m3fn, device="cuda:0") for n in (9, 200))
+s, t = (torch.zeros((1, n, 4), dtype=torch.float8_e8m0fnu, device="cuda:0") for n in (9, 200))
+torch.cuda.synchronize()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        ops.gemm_fp8(a, s, b, t)
+except ops.KernelError as e:
+    print("refused" if "must not be captured" in str(e) else e)
+x, w = (ops.quantize_fp8(torch.randn(n, 256, device="cuda:0")) for n in (9, 200))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = ops.gemm_fp8(*x, *w)
+ops.check_tc_error("cuda:0")
+ops.tc_error_flag("cuda:0").fill_(1)
+g.replay()
+torch.cuda.synchronize()
+try:
+    ops.check_tc_error("cuda:0")
+    print("lost")
+except ops.KernelError:
+    print("reported", bool((y == ops.gemm_fp8(*x, *w)).all()))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.split() == ["refused", "reported", "True"], run.stdout + run.stderr[-2000:]
