@@ -18,13 +18,12 @@
 constexpr int F8_THREADS = 256;
 enum F8Way : int { F8_RUNS = 0, F8_FOURS = 1, F8_PAIRS = 2, F8_ONES = 3 };
 
-// Sixteen consecutive numbers from a 32-byte boundary, two in a register, and apart.
-__device__ __forceinline__ void f8_load16(const __nv_bfloat16* p, uint32_t (&r)[8]) {
+// Sixteen consecutive numbers from a 32-byte boundary.
+__device__ __forceinline__ void f8_load16(const __nv_bfloat16* p, float (&v)[16]) {
+  uint32_t r[8];
   asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "l"(p));
-}
-__device__ __forceinline__ void f8_apart16(const uint32_t (&r)[8], float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     v[2 * i] = __uint_as_float(r[i] << 16);
@@ -217,11 +216,7 @@ f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, cons
       const int at = (2 * blockIdx.y + h) * F8_WORD, left = live ? o.width - at : 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[h][i] = 0.f;
-      uint32_t pairs[8];
-      if (16 * lane < left) {
-        f8_load16(xr + at + 16 * lane, pairs);
-        f8_apart16(pairs, v[h]);
-      }
+      if (16 * lane < left) f8_load16(xr + at + 16 * lane, v[h]);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -234,10 +229,13 @@ f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, cons
 }
 
 // ---- the gated unit -------------------------------------------------------------------------------------------------
-// GatedUnit in fewer instructions: e^x as 2^(x log2 e) and the quotient by a reciprocal, both approximate. Off by some 2^-21 of itself, and
-// by |alpha gate| 2^-23 more for a negative gate (the exponent's own rounding), before a rounding of 2^-4. PLAIN is silu(gate) * up. What
-// bounded the kernel were these instructions beside the memory: 2,048 rows of 12,288 took 33 us with expf and a division, 24.5 with expf
-// and a corrected reciprocal, 20.1 with this, 20.5 with the look for gates far below zero (19.5 at 6.45 TB/s).
+// GatedUnit in fewer instructions: with t = alpha gate and e = e^(-|t| / 2) the sigmoid of t is 1 / (1 + e^2), times e^2 where t < 0: there
+// gate and up are multiplied by e each, so that no product on the way leaves float32 where the result does not (a single
+// e^2, or 1 + e^-t, ends at t = -87). The power and the reciprocal are approximate: off by some 2^-21 of itself, and by |t| 2^-23 more
+// for t < 0 (the exponent's own rounding), before a rounding of 2^-4; 0 for t < -174, where e^t is below 2^-251. PLAIN is silu(gate) * up.
+// What bounded the kernel were these instructions beside the memory: 2,048 rows of 12,288 took 33 us with expf and a division,
+// 20.1 as gate / (1 + e^-t), 20.4 with this (19.5 at 6.45 TB/s). A look for gates below -87 in place of it took 20.6 and, where one word in a
+// hundred holds one, 21.7 (those numbers again) or 27 (their word again).
 constexpr float F8_LOG2E = 1.44269504088896f;      // log2(e)
 // The smaller (larger) of two; a NaN where either is one, so that a limit hides none.
 __device__ __forceinline__ float f8_min(float a, float b) {
@@ -250,73 +248,29 @@ __device__ __forceinline__ float f8_max(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// `most`: the largest 1 + e^-(alpha gate) so far. From 2^126 (e^87.3) on the reciprocal is 0. A word that holds an alpha gate below F8_LOW,
-// perhaps one just above, is made by f8_unit_again, which takes another way for those below: what becomes of a number does not
-// depend on its neighbours.
-constexpr float F8_MOST = 0x1p125f, F8_LOW = -87.0f;
-template <bool PLAIN>
-__device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, float up, float& most) {
-  const float g = PLAIN ? gate : f8_min(gate, unit.limit), u = PLAIN ? up : f8_min(f8_max(up, -unit.limit), unit.limit);
+// SELECT: e or 1 for every number, which float32 rows and numbers one by one hold in fewer registers (float32, 3,000 rows of 4,112: 18.9
+// us; 20.7 by branches, which take bfloat16 runs 20.4 where selecting takes 20.9).
+template <bool PLAIN, bool SELECT>
+__device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, float up) {
+  float g = PLAIN ? gate : f8_min(gate, unit.limit), u = PLAIN ? up : f8_min(f8_max(up, -unit.limit), unit.limit) + unit.shift;
+  const float y = g * (PLAIN ? 0.5f * F8_LOG2E : 0.5f * F8_LOG2E * unit.alpha);
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * (PLAIN ? -F8_LOG2E : -F8_LOG2E * unit.alpha)));
-  e += 1.0f, most = fmaxf(most, e);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e));
-  return g * r * (PLAIN ? u : u + unit.shift);
-}
-// Whether one of sixteen bfloat16 gates, two in a register, may be as far below zero: fewer instructions than `most`, which the
-// compiler leaves out where nothing reads it (2,048 rows of 12,288 20.5 us, 20.6 with `most`, 20.1 without either; clamped 22.2,
-// 23.4 and 21.2).
-template <bool PLAIN>
-__device__ __forceinline__ bool f8_far(const GatedUnit& unit, const uint32_t (&r)[8]) {
-  __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __nv_bfloat162 g = *reinterpret_cast<const __nv_bfloat162*>(&r[i]);
-    m = PLAIN ? __hmin2(m, g) : __hmax2(m, __habs2(g));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-fabsf(y)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, e, 1.0f)));
+  if constexpr (SELECT) {
+    e = y < 0.0f ? e : 1.0f;
+    g *= e, u *= e;
+  } else if (y < 0.0f) {
+    g *= e, u *= e;
   }
-  const float lo = __low2float(m), hi = __high2float(m);
-  return (PLAIN ? fminf(lo, hi) : -fabsf(fmaxf(lo, hi) * unit.alpha)) < F8_LOW;
-}
-// A warp's 512 numbers where some alpha gate = t is below F8_LOW: there e^t / (1 + e^t) with e^t as a square, whose root enters before
-// the other factor and after it, so that no product on the way leaves float32 where the result does not. Number by number and
-// out of line: such gates are rare, and this beside the usual way in line took 21.6 us in place of 20.1.
-template <typename T>
-static __device__ __noinline__ void f8_unit_again(const T* row, int block, int at, int left, GatedUnit unit, uint8_t* q,
-                                                  uint32_t* word) {
-  const int lane = threadIdx.x & 31;
-  uint32_t w = 0;
-#pragma unroll 1
-  for (int j = 0; j < 4; ++j) {
-    float v[4], top = 0.f, most = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = 128 * j + 32 * i + lane, c = at + n;
-      v[i] = 0.f;
-      if (n >= left) continue;
-      const T* p = row + c + c / block * block;
-      const float g = f8_min(to_float(p[0]), unit.limit), u = f8_min(f8_max(to_float(p[block]), -unit.limit), unit.limit);
-      const float t = g * unit.alpha;
-      float e;
-      asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t * (0.5f * F8_LOG2E)));      // (1 + e^t is 1)
-      v[i] = t < F8_LOW ? g * e * (u + unit.shift) * e : f8_unit<false>(unit, g, u, most);
-      top = fmaxf(top, fabsf(v[i]));
-    }
-    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    const uint32_t byte = f8_scale_byte(top);
-    const float inv = f8_inverse(byte);
-    w |= byte << (8 * j);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (128 * j + 32 * i + lane < left) q[128 * j + 32 * i + lane] = (uint8_t)f8_pack2_any(v[i] * inv, 0.f);
-  }
-  if (lane == 0) *word = w;
+  return g * r * u;
 }
 
 // gate(c): where column c's gate is; its up is `block` further. A lane's sixteen (runs) or four (fours) columns lie within a run of
 // `block`; pairs: the layout is plain.
 template <typename T, int WAY, bool PLAIN, bool FULL, typename Gate>
-__device__ __forceinline__ void f8_unit_word(const T* row, const Gate& gate, int block, int at, int left, const GatedUnit& unit,
-                                             uint8_t* q, uint32_t* word) {
+__device__ __forceinline__ void f8_unit_word(const Gate& gate, int block, int at, int left, const GatedUnit& unit, uint8_t* q,
+                                             uint32_t* word) {
   const int lane = threadIdx.x & 31;
   float g[16], v[16];
 #pragma unroll
@@ -328,21 +282,18 @@ __device__ __forceinline__ void f8_unit_word(const T* row, const Gate& gate, int
     f8_load<WAY, FULL>([&](int c) { return gate(at + c); }, left, g);
     f8_load<WAY, FULL>([&](int c) { return gate(at + c) + block; }, left, v);
   }
-  float most = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int c = WAY == F8_FOURS ? 128 * (i / 4) + 4 * lane : WAY == F8_PAIRS ? 64 * (i / 2) + 2 * lane + i % 2 : 32 * i + lane;
-    v[i] = FULL || c < left ? f8_unit<PLAIN>(unit, g[i], v[i], most) : 0.f;      // (the unit of zeros need not be zero)
+    v[i] = FULL || c < left ? f8_unit<PLAIN, sizeof(T) == 4 || WAY == F8_ONES>(unit, g[i], v[i]) : 0.f;      // (the unit of zeros need not be zero)
   }
-  if (__any_sync(0xffffffffu, most > F8_MOST))
-    f8_unit_again<T>(row, block, at, left, unit, q, word);
-  else
-    f8_store<WAY, FULL>(v, q, left, word);
+  f8_store<WAY, FULL>(v, q, left, word);
 }
 
-// `shift`: block = 2^shift, or -1.
+// `shift`: block = 2^shift, or -1. Blocks an SM at the least, by ways (one B200, eight | six): runs 20.4 | 20.8 us; pairs, 4,000 rows of
+// 1,001, 6.5 | 5.8; numbers one by one, 3,000 rows of 4,095, 43.5 with six, 41.4 with five.
 template <typename T, int WAY, bool PLAIN>
-__global__ void __launch_bounds__(F8_THREADS)
+__global__ void __launch_bounds__(F8_THREADS, sizeof(T) == 4 ? 4 : WAY == F8_RUNS ? 8 : WAY == F8_ONES ? 5 : 6)
 f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shift, const GatedUnit unit, const F8Rows o) {
   pdl_launch_dependents();
   pdl_wait();
@@ -356,30 +307,22 @@ f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shi
   const bool whole = block == o.width;
   auto gate = [&](int c) { return row + c + (whole ? 0 : shift >= 0 ? c >> shift << shift : c / block * block); };
   if constexpr (WAY == F8_RUNS) {
-    float v[16], most = 0.f;
-    bool far = false;
+    float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.f;
     if (16 * lane < left) {
       float g[16];
-      uint32_t r[8];
       const T* p = gate(at + 16 * lane);
-      f8_load16(p, r);
-      far = f8_far<PLAIN>(unit, r);
-      f8_apart16(r, g);
-      f8_load16(p + block, r);
-      f8_apart16(r, v);
+      f8_load16(p, g);
+      f8_load16(p + block, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = f8_unit<PLAIN>(unit, g[i], v[i], most);
+      for (int i = 0; i < 16; ++i) v[i] = f8_unit<PLAIN, false>(unit, g[i], v[i]);
     }
-    if (__any_sync(0xffffffffu, far))
-      f8_unit_again<T>(row, block, at, left, unit, q, w);
-    else
-      f8_store_runs(v, 16 * lane < left ? q + 16 * lane : nullptr, w);
+    f8_store_runs(v, 16 * lane < left ? q + 16 * lane : nullptr, w);
   } else if (left >= F8_WORD) {
-    f8_unit_word<T, WAY, PLAIN, true>(row, gate, block, at, left, unit, q, w);
+    f8_unit_word<T, WAY, PLAIN, true>(gate, block, at, left, unit, q, w);
   } else {
-    f8_unit_word<T, WAY, PLAIN, false>(row, gate, block, at, left, unit, q, w);
+    f8_unit_word<T, WAY, PLAIN, false>(gate, block, at, left, unit, q, w);
   }
 }
 
