@@ -234,7 +234,7 @@ f8_quantize_kernel(const T* __restrict__ x, long long x_stride, int x_rows, cons
 // e^2, or 1 + e^-t, ends at t = -87). The power and the reciprocal are approximate: off by some 2^-21 of itself, and by |t| 2^-23 more
 // for t < 0 (the exponent's own rounding), before a rounding of 2^-4; 0 for t < -174, where e^t is below 2^-251. PLAIN is silu(gate) * up.
 // What bounded the kernel were these instructions beside the memory: 2,048 rows of 12,288 took 33 us with expf and a division,
-// 20.1 as gate / (1 + e^-t), 20.4 with this (19.5 at 6.45 TB/s). A look for gates below -87 in place of it took 20.6 and, where one word in a
+// 20.1 as gate / (1 + e^-t), 20.8 with this (19.5 at 6.45 TB/s). A look for gates below -87 in place of it took 20.6 and, where one word in a
 // hundred holds one, 21.7 (those numbers again) or 27 (their word again).
 constexpr float F8_LOG2E = 1.44269504088896f;      // log2(e)
 // The smaller (larger) of two; a NaN where either is one, so that a limit hides none.
@@ -249,7 +249,7 @@ __device__ __forceinline__ float f8_max(float a, float b) {
   return r;
 }
 // SELECT: e or 1 for every number, which float32 rows and numbers one by one hold in fewer registers (float32, 3,000 rows of 4,112: 18.9
-// us; 20.7 by branches, which take bfloat16 runs 20.4 where selecting takes 20.9).
+// us; 20.7 by branches, which take bfloat16 runs 20.8 where selecting takes 21.0).
 template <bool PLAIN, bool SELECT>
 __device__ __forceinline__ float f8_unit(const GatedUnit& unit, float gate, float up) {
   float g = PLAIN ? gate : f8_min(gate, unit.limit), u = PLAIN ? up : f8_min(f8_max(up, -unit.limit), unit.limit) + unit.shift;
@@ -290,10 +290,11 @@ __device__ __forceinline__ void f8_unit_word(const Gate& gate, int block, int at
   f8_store<WAY, FULL>(v, q, left, word);
 }
 
-// `shift`: block = 2^shift, or -1. Blocks an SM at the least, by ways (one B200, eight | six): runs 20.4 | 20.8 us; pairs, 4,000 rows of
-// 1,001, 6.5 | 5.8; numbers one by one, 3,000 rows of 4,095, 43.5 with six, 41.4 with five.
+// `shift`: block = 2^shift, or -1. Blocks an SM at the least (one B200): with eight in place of six, runs of 2,048 x 12,288 take
+// 20.4 us in place of 20.8 in a burst, but 23.4 in place of 22.5 where calls follow one another for seconds under the power limit;
+// pairs, 4,000 rows of 1,001, 6.5 and 5.8; numbers one by one, 3,000 rows of 4,095, 43.5 with six, 41.4 with five.
 template <typename T, int WAY, bool PLAIN>
-__global__ void __launch_bounds__(F8_THREADS, sizeof(T) == 4 ? 4 : WAY == F8_RUNS ? 8 : WAY == F8_ONES ? 5 : 6)
+__global__ void __launch_bounds__(F8_THREADS, sizeof(T) == 4 ? 4 : WAY == F8_ONES ? 5 : 6)
 f8_unit_kernel(const T* __restrict__ gu, long long gu_stride, int block, int shift, const GatedUnit unit, const F8Rows o) {
   pdl_launch_dependents();
   pdl_wait();
