@@ -43,8 +43,8 @@ def _add_common(p: argparse.ArgumentParser) -> None:
     p.add_argument("--prompt-len", type=int, default=16, help="length of a random prompt when no prompt is given")
     p.add_argument("--prompt-seed", type=int, default=0)
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
-    p.add_argument("--products", choices=["stored", "fp8"], default="stored", help="fp8: attention projections, feed-forwards and "
-                   "experts in 8 bits with a scale for each block of 128 (bfloat16 only)")
+    p.add_argument("--products", choices=["stored", "fp8"], default="stored", help="fp8: projections of grouped-query and scored "
+                   "attention, feed-forwards and experts in 8 bits with a scale for each block of 128 (bfloat16 only)")
     p.add_argument("--block-pool-size", type=int, default=1024, help="pages in the cache pool")
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--seed", type=int, default=0, help="seed of the sampler's draws")

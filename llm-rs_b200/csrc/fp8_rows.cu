@@ -6,12 +6,12 @@
 //           bytes, a store of 16); a block's maximum is the maximum over 8 neighbouring lanes
 //   fours   rows of whole fours that start on the boundaries of four numbers: 4 consecutive numbers of each of the four blocks
 //           (loads of 16 bytes of float32, of 8 of bfloat16; stores of 4); a block's maximum is the maximum over the warp. float32
-//           goes this way: a norm's loads and stores of 32 bytes a lane took 41.1 us, those of 16 35.3 (4,001 rows of 5,120), a
-//           float32 unit 21.7 and 18.3 (3,000 rows of 4,112)
+//           goes this way: a norm's loads and stores of 32 bytes a lane took 41.1 us where those of 16 took 35.3 (4,001 rows of
+//           5,120, sums in float32), a float32 unit 21.7 and 18.3 (3,000 rows of 4,112; 18.9 since its gates may be anything)
 //   pairs   all other rows: aligned pairs, 32 neighbours a load, moved over by a number where the row starts inside one. Rows of
 //           4,095 bfloat16 numbers (8,000 of them) took 25.9 us by unaligned fours, 36 one by one, 20.9 so (15.3 at 6.45 TB/s)
 //   ones    every 32nd number: the norm of such rows, whose sums go back where the numbers came from (2,000 rows of 5,001: 32.3 us by
-//           unaligned fours, 23.7 so), and units whose columns alternate by a number that is not a multiple of four
+//           unaligned fours, 25.0 so), and units whose columns alternate by a number that is not a multiple of four
 // Words that lie whole within a row go without a comparison a number: on odd rows the instructions are what bounds.
 #include "fp8.cuh"
 

@@ -37,8 +37,8 @@ class EngineConfig:
     # Queue the next step on the GPU before the last one's tokens are read back (they feed
     # the next step on the device); ``step()`` then reports a step's tokens one call later.
     async_steps: bool = True
-    # "stored", or "fp8": attention projections, feed-forwards and experts in 8 bits (bfloat16 engines; the weights are
-    # quantised as they are loaded, the activations in every step).
+    # "stored", or "fp8": the projections of grouped-query and scored attention, feed-forwards and experts in 8 bits (bfloat16
+    # engines; the weights are quantised as they are loaded, the activations in every step).
     products: str = "stored"
 
 

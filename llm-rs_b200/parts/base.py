@@ -26,8 +26,9 @@ class Runtime:
     device: torch.device
     act_dtype: torch.dtype          # bfloat16 or float32: type of activations and of the cache
     max_positions: int              # positions 0 .. max_positions-1 can occur
-    # "stored": products of the weights as they are; "fp8": the attention projections, the feed-forward's and the experts'
-    # products of bfloat16 weights in 8 bits (``parts.linear.Fp8Linear``). Everything else stays as it is stored.
+    # "stored": products of the weights as they are; "fp8": the projections of grouped-query and scored attention, the
+    # feed-forward's and the experts' products of bfloat16 weights in 8 bits (``parts.linear.Fp8Linear``). Everything else, latent
+    # attention and the recurrences' projections among it, stays as it is stored.
     products: str = "stored"
 
     @property
