@@ -86,7 +86,9 @@ class SwiGLU(FeedForward):
         # 64 tokens), for many the persistent tcgen05 kernel on pairs of SMs (2,048 tokens: 261 against 271 + 20 us).
         if self.block and x.dtype == torch.bfloat16 and self.gate_up.tc_enabled() and FUSE_GATE_UP:
             act = ops.gemm_bf16(x, self.gate_up.weight, epilogue="silu_mul", then=self.gate_up.next_weight, unit=self.unit)
-        elif isinstance(self.down, Fp8Linear):      # the unit's result goes into the next product in 8 bits
+        elif isinstance(self.down, Fp8Linear):
+            # The unit's result goes into the next product in 8 bits. Gate and up lie between the two kernels in bfloat16: half the
+            # bytes of float32 written and read, for a rounding of 2^-8 of each before one of 2^-4 of their unit.
             act = Rows8(*ops.silu_mul_fp8(self.gate_up.forward(x), block=self.block, unit=self.unit))
         else:
             act = ops.silu_mul(self.gate_up.forward(x), block=self.block, unit=self.unit)

@@ -195,6 +195,7 @@ class MixtureOfExperts(FeedForward):
         rows = torch.empty((n_rows, self.hidden_size), dtype=torch.float32, device=x.device)
         if self.fp8:
             w, scales, w_down, down_scales = self.fp8
+            # Gate and up lie between the product and the unit in bfloat16, as the dense feed-forward's do.
             gate_up = torch.empty((n_rows, w.size(1)), dtype=self.act_dtype, device=x.device)
             ops.gemm_fp8_grouped(*ops.quantize_fp8(x, src_token), w, scales, gate_up, tiles, n_tiles, tile_rows)
             act8 = ops.silu_mul_fp8(gate_up, block=self.block, unit=(self.limit, self.alpha, self.up_shift))
